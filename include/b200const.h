@@ -52,6 +52,10 @@ extern "C" {
 #define B200C_F32 B200C_DTYPE(B200C_CLS_FLOAT, 32)
 #define B200C_F16 B200C_DTYPE(B200C_CLS_FLOAT, 16)
 #define B200C_BF16 B200C_DTYPE(B200C_CLS_BFLOAT, 16)
+/* 4-bit float (1 sign, 2 exponent, 1 fraction bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives),
+ * two to a byte, low nibble first.  No counterpart in the reference: the element type of the
+ * block-scaled matrices below.                                                       */
+#define B200C_F4E2M1 B200C_DTYPE(B200C_CLS_FLOAT, 4)
 #define B200C_I1 B200C_DTYPE(B200C_CLS_INT, 1)
 #define B200C_UI1 B200C_DTYPE(B200C_CLS_UINT, 1)
 #define B200C_I4 B200C_DTYPE(B200C_CLS_INT, 4)
@@ -340,6 +344,67 @@ B200C_API int b200c_btc_compress_inplace_batch(b200c_ctx* ctx, int count, void* 
 B200C_API int b200c_btc_compress_inplace_begin(b200c_ctx* ctx, int count, void* const* bufs_dev, const size_t* sizes,
                                                int* ticket);
 B200C_API int b200c_btc_compress_inplace_end(b200c_ctx* ctx, int ticket, size_t* out_sizes, int32_t* compressed);
+
+/* ---- block-scaled 4-bit matrices --------------------------------------------------------
+ * (No counterpart in the reference, whose narrowest weights are int4 with one scale per channel.)
+ *
+ * A matrix of rows x cols in 4 bits: e2m1 codes and one scale per block of neighbours in a row.
+ *   B200C_MXFP4: blocks of 32; scale 2^X, X = floor(log2(max|v|)) - 2, at least -127, stored as the
+ *                byte X + 127 (e8m0).
+ *   B200C_NVFP4: blocks of 16; scale = e4m3(min(448, max|v| / (6 t))), to nearest even, and one
+ *                32-bit factor t of the whole matrix.
+ * With d = the block's scale (times t, rounded to 32 bits):
+ *   code = e2m1(v / d): nearest, ties to even, magnitudes above 6 become 6, the sign of v is kept.
+ * 6 t, max|v| / (6 t) and v / d are rounded to 32 bits on the way; where t is a power of two, as the
+ * one that the library finds, no such rounding changes a scale or a code.  Blocks of their own kind:
+ *   a block whose d is 0 has the codes 0; a block that holds a NaN or an infinity has the scale NaN
+ *   (0xFF / 0x7F) and the codes 0.  What a code stands for is code * d: NaN for such a block.
+ *
+ * Storage.  codes: two to a byte, low nibble first, row r at codes + r * ld.  A row is padded with
+ * zero codes to a whole number of 32 elements, so ld is a multiple of 16 and at least
+ * 16 * ceil(cols / 32); codes is 16-byte aligned.
+ * scales: one byte per block.  B200C_MX_SCALES_ROWS: [rows][blocks], blocks = ceil(cols / block).
+ * B200C_MX_SCALES_TILED, which the product reads: tiles of 128 rows x 4 blocks, 512 bytes each,
+ * ordered [row tile][block tile]; inside a tile row r, block b at (r % 32) * 16 + (r / 32) * 4 + b.
+ * Rows and blocks that only fill a tile up have the scale byte 0.  16-byte aligned.
+ * tensor_scale (B200C_NVFP4; not read for B200C_MXFP4): two floats in device memory, t and the
+ * largest finite magnitude of the matrix.
+ *
+ * b200c_mx_sizes: the smallest ld, and the bytes of codes (with that ld) and scales.  Host code.
+ *
+ * The other calls queue work on the context's stream and return; all pointers are device pointers.
+ * They allocate nothing and keep nothing, so they may be captured into a CUDA graph, and leave the
+ * calling thread's current device as it was.  Outputs must not overlap inputs or one another
+ * (refused).  Empty matrices are fine: nothing but what the shapes say is written.
+ *
+ * b200c_mx_quantize: src (f16, bf16 or f32; rows and cols of `out`, src_ld elements between rows) ->
+ * out.  All bytes of the codes' padded rows (not those up to a larger ld) and of the scales are written.  t of
+ * B200C_NVFP4 is the smallest power of two, at least 2^-126, with max|V| <= 2688 t over the finite values
+ * (2688 = 6 * 448; 1 for a matrix without a finite non-zero value), and both floats of tensor_scale are
+ * written; with B200C_MX_SCALE_GIVEN t is read from tensor_scale[0] instead (positive and finite, or
+ * every scale becomes NaN) and nothing is written there.  `values` (may be NULL): what the codes stand
+ * for, in the type of src, values_ld elements between rows.
+ *
+ * b200c_mx_dequantize: what the codes of `m` stand for -> out (f16, bf16 or f32, rounded from 32 bits).   */
+#define B200C_MXFP4 1
+#define B200C_NVFP4 2
+#define B200C_MX_SCALES_ROWS 0
+#define B200C_MX_SCALES_TILED 1
+#define B200C_MX_SCALE_GIVEN 1
+typedef struct b200c_mx_matrix {
+    int32_t format;
+    int32_t scale_layout;
+    int64_t rows, cols;
+    int64_t ld; /* bytes */
+    void* codes;
+    void* scales;
+    float* tensor_scale;
+} b200c_mx_matrix;
+B200C_API int b200c_mx_sizes(int32_t format, int32_t scale_layout, int64_t rows, int64_t cols, int64_t* ld,
+                             size_t* code_bytes, size_t* scale_bytes);
+B200C_API int b200c_mx_quantize(b200c_ctx* ctx, const void* src, int32_t src_dtype, int64_t src_ld,
+                                const b200c_mx_matrix* out, void* values, int64_t values_ld, int flags);
+B200C_API int b200c_mx_dequantize(b200c_ctx* ctx, const b200c_mx_matrix* m, void* out, int32_t out_dtype, int64_t out_ld);
 
 /* ---- splat detection -------------------------------------------------------------
  * "All elements equal" test of a raw buffer: detectSplatElementWise, which the reference runs when

@@ -21,6 +21,7 @@ def dtype_class(dt):
     return (dt >> 8) & 0xFF
 
 
+F4E2M1 = DTYPE(CLS_FLOAT, 4)
 F64, F32, F16 = DTYPE(CLS_FLOAT, 64), DTYPE(CLS_FLOAT, 32), DTYPE(CLS_FLOAT, 16)
 BF16 = DTYPE(CLS_BFLOAT, 16)
 I1, UI1 = DTYPE(CLS_INT, 1), DTYPE(CLS_UINT, 1)
@@ -59,6 +60,9 @@ OK, NOT_SMALLER = 0, 1
 ERR_INVALID, ERR_THROW, ERR_CUDA, ERR_NOMEM, ERR_CAPACITY, ERR_UNSUPPORTED = -1, -2, -3, -4, -5, -6
 
 FOLD_ASYNC = 1
+MXFP4, NVFP4 = 1, 2
+MX_SCALES_ROWS, MX_SCALES_TILED = 0, 1
+MX_SCALE_GIVEN = 1
 NOALLOC_MAX_INPUT = 16 << 20
 
 
@@ -124,6 +128,19 @@ class b200c_copy_seg(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("n", C.c_size_t)]
 
 
+class b200c_mx_matrix(C.Structure):
+    _fields_ = [
+        ("format", C.c_int32),
+        ("scale_layout", C.c_int32),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("ld", C.c_int64),
+        ("codes", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("tensor_scale", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes) of every symbol include/b200const.h declares
 _P = C.POINTER
 SYMBOLS = {
@@ -159,6 +176,10 @@ SYMBOLS = {
     "b200c_btc_compress_inplace_end": (C.c_int, [C.c_void_p, C.c_int, _P(C.c_size_t), _P(C.c_int32)]),
     "b200c_synth_fill": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_double, C.c_double,
                                    C.c_uint64, C.c_uint64]),
+    "b200c_mx_sizes": (C.c_int, [C.c_int32, C.c_int32, C.c_int64, C.c_int64, _P(C.c_int64), _P(C.c_size_t), _P(C.c_size_t)]),
+    "b200c_mx_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, _P(b200c_mx_matrix), C.c_void_p, C.c_int64,
+                                    C.c_int]),
+    "b200c_mx_dequantize": (C.c_int, [C.c_void_p, _P(b200c_mx_matrix), C.c_void_p, C.c_int32, C.c_int64]),
     "b200c_detect_splat": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int, _P(C.c_int)]),
     "b200c_digest64_batch": (C.c_int, [C.c_void_p, C.c_int, _P(C.c_void_p), _P(C.c_size_t), _P(C.c_uint64)]),
     "b200c_ipc_export": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, _P(b200c_ipc_handle)]),

@@ -540,6 +540,27 @@ class CudaBackend:
         raise_for(self.lib.b200c_dev_memset(self.ctx, dev_ptr, 0, int(nbytes)), self._err())
         self.synchronize()
 
+    def set_stream(self, stream):
+        """All later work of this backend goes to `stream` (a cudaStream_t as an integer, e.g. a torch stream's
+        cuda_stream; 0 is CUDA's default stream).  None: back to the backend's own stream."""
+        handle = None if stream is None else int(stream) or 1  # cudaStreamLegacy: a null handle means the own stream
+        raise_for(self.lib.b200c_set_stream(self.ctx, handle), self._err())
+
+    # ---- block-scaled 4-bit matrices (npu_plugin_b200.mx.MxMatrix; device pointers, on the backend's stream)
+    def mx_quantize(self, src, dtype, src_ld, out, tensor_scale_given=False, values=None, values_ld=0):
+        """src (rows x cols of `out`, f16/bf16/f32, src_ld elements between rows) -> the codes and scales of `out`;
+        `values` receives what they stand for, in the type of src."""
+        rc = self.lib.b200c_mx_quantize(self.ctx, src, dtype, src_ld, C.byref(out.c), values, values_ld,
+                                        A.MX_SCALE_GIVEN if tensor_scale_given and out.c.format == A.NVFP4 else 0)
+        if rc:
+            raise_for(rc, self._err())
+
+    def mx_dequantize(self, m, out, dtype, out_ld):
+        """What the codes of `m` stand for -> out (f16/bf16/f32, out_ld elements between rows)."""
+        rc = self.lib.b200c_mx_dequantize(self.ctx, C.byref(m.c), out, dtype, out_ld)
+        if rc:
+            raise_for(rc, self._err())
+
     def synth_fill(self, dev_ptr, count, dtype, dist, p0, p1, seed, stream_id):
         raise_for(self.lib.b200c_synth_fill(self.ctx, dev_ptr, int(count), dtype, dist, p0, p1, seed, stream_id), self._err())
 

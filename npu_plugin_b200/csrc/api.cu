@@ -1,6 +1,7 @@
 // C ABI of the library (include/b200const.h): context management, memory helpers and the entry
 // points that drive the planner and the codec.  No exception crosses this file's boundary.
 #include "../../include/b200const.h"
+#include "mx.h"
 #include "plan.h"
 
 #include <algorithm>
@@ -989,6 +990,58 @@ int b200c_btc_compress_inplace_end(b200c_ctx* h, int ticket, size_t* out_sizes, 
             out_sizes[i] = res[i].size;
             if (compressed) compressed[i] = res[i].notSmaller ? 0 : 1;
         }
+    });
+}
+
+// ---------------------------------------------------------------------------- block-scaled 4-bit matrices
+namespace {
+// These calls use neither the arena nor the staging buffers, so nothing is rewound for them, and they
+// leave the calling thread's device as it was.
+struct MxScope {
+    std::unique_lock<std::mutex> lock;
+    int before = -1;
+    explicit MxScope(Context* ctx): lock(ctx->mu) {
+        B2_CUDA(cudaGetDevice(&before));
+        if (before == ctx->device) {
+            before = -1;
+        } else {
+            B2_CUDA(cudaSetDevice(ctx->device));
+        }
+    }
+    ~MxScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+}  // namespace
+
+int b200c_mx_sizes(int32_t format, int32_t scale_layout, int64_t rows, int64_t cols, int64_t* ld, size_t* code_bytes,
+                   size_t* scale_bytes) {
+    return guarded([&] {
+        mxCheckShape(format, scale_layout, rows, cols);
+        if (ld) *ld = mxPitch(cols);
+        if (code_bytes) *code_bytes = static_cast<size_t>(rows * mxPitch(cols));
+        if (scale_bytes) *scale_bytes = static_cast<size_t>(mxScaleBytes(format, scale_layout, rows, cols));
+    });
+}
+
+int b200c_mx_quantize(b200c_ctx* h, const void* src, int32_t src_dtype, int64_t src_ld, const b200c_mx_matrix* out, void* values,
+                      int64_t values_ld, int flags) {
+    return guarded([&] {
+        mxCheckQuantize(src, src_dtype, src_ld, out, values, values_ld, flags);
+        if (!h) throw BadArg("null context");
+        Context* ctx = reinterpret_cast<Context*>(h);
+        MxScope scope(ctx);
+        launchMxQuantize(ctx, src, src_dtype, src_ld, *out, values, values_ld, (flags & B200C_MX_SCALE_GIVEN) != 0);
+    });
+}
+
+int b200c_mx_dequantize(b200c_ctx* h, const b200c_mx_matrix* m, void* out, int32_t out_dtype, int64_t out_ld) {
+    return guarded([&] {
+        mxCheckDequantize(m, out, out_dtype, out_ld);
+        if (!h) throw BadArg("null context");
+        Context* ctx = reinterpret_cast<Context*>(h);
+        MxScope scope(ctx);
+        launchMxDequantize(ctx, *m, out, out_dtype, out_ld);
     });
 }
 

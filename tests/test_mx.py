@@ -1,0 +1,263 @@
+"""Block-scaled 4-bit matrices: quantisation and its inverse against a 64-bit oracle, byte for byte, and the refusals
+of their entry points.  The refusals run without a device: every argument is checked before the context is."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import mx_oracle as O
+from npu_plugin_b200 import _cabi as A
+from npu_plugin_b200 import mx
+
+torch = pytest.importorskip("torch")
+
+FORMATS = [A.MXFP4, A.NVFP4]
+LAYOUTS = [A.MX_SCALES_ROWS, A.MX_SCALES_TILED]
+TYPES = {A.F16: torch.float16, A.BF16: torch.bfloat16, A.F32: torch.float32}
+CANARY = 0xA5
+
+
+# --------------------------------------------------------------------------- host side
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols", [(0, 0), (1, 1), (1, 32), (127, 33), (128, 64), (129, 4096), (5, 1003)])
+def test_sizes(fmt, rows, cols):
+    blocks = -(-cols // O.BLOCK[fmt])
+    assert mx.sizes(fmt, rows, cols, A.MX_SCALES_ROWS) == (-(-cols // 32) * 16, rows * -(-cols // 32) * 16, rows * blocks)
+    tiles = -(-rows // 128) * -(-blocks // 4)
+    assert mx.sizes(fmt, rows, cols) == (-(-cols // 32) * 16, rows * -(-cols // 32) * 16, tiles * 512)
+
+
+def matrix(**kw):
+    a = dict(fmt=A.NVFP4, rows=64, cols=64, codes=0x10000, scales=0x20000, tensor_scale=0x30000)
+    a.update(kw)
+    return mx.MxMatrix(**a)
+
+
+def refused(call, *args):
+    lib = A.load()
+    assert getattr(lib, call)(None, *args) == A.ERR_INVALID
+    return lib.b200c_last_error().decode()
+
+
+QUANTIZE = dict(src=0x100000, dtype=A.F16, ld=64, values=None, values_ld=0, flags=0)
+
+
+@pytest.mark.parametrize("change,said", [
+    (dict(), "null context"),
+    (dict(dtype=A.F64), "element type"), (dict(dtype=A.SI8), "element type"),
+    (dict(ld=63), "fewer elements"), (dict(src=None), "source: null"), (dict(src=0x100001), "not aligned"),
+    (dict(values=0x200000, values_ld=63), "values: fewer"), (dict(values=0x200001, values_ld=64), "values: not aligned"),
+    (dict(values=0x100000, values_ld=64), "overlaps source"), (dict(values=0x10000, values_ld=64), "overlaps codes"),
+    (dict(src=0x10040), "codes overlaps source"), (dict(src=0x20000), "scales overlaps source"),
+    (dict(flags=2), "unknown flags"), (dict(ld=1 << 60), "too large"),
+    (dict(m=dict(fmt=3)), "format"), (dict(m=dict(layout=2)), "layout"), (dict(m=dict(rows=-1)), "negative"),
+    (dict(m=dict(cols=1 << 31)), "too large"), (dict(m=dict(ld=16)), "multiple of 16"), (dict(m=dict(ld=40)), "multiple of 16"),
+    (dict(m=dict(codes=None)), "null pointer"), (dict(m=dict(scales=None)), "null pointer"),
+    (dict(m=dict(codes=0x10008)), "codes have to be 16-byte"), (dict(m=dict(scales=0x20004)), "tiled scales"),
+    (dict(m=dict(tensor_scale=None)), "needs a tensor scale"), (dict(m=dict(tensor_scale=0x30002)), "tensor scale is not"),
+    (dict(m=dict(scales=0x10400)), "codes overlaps scales"), (dict(m=dict(tensor_scale=0x10000)), "overlaps tensor scale"),
+    (dict(m=dict(fmt=A.MXFP4), flags=A.MX_SCALE_GIVEN), "no tensor scale"),
+])
+def test_quantize_refusals(change, said):
+    a = dict(QUANTIZE, **{k: v for k, v in change.items() if k != "m"})
+    kw = change.get("m", {})
+    kw.setdefault("ld", 32)
+    m = matrix(**kw)
+    assert said in refused("b200c_mx_quantize", a["src"], a["dtype"], a["ld"], C.byref(m.c), a["values"], a["values_ld"], a["flags"])
+
+
+@pytest.mark.parametrize("change,said", [
+    (dict(), "null context"), (dict(dtype=A.UI8), "element type"), (dict(ld=60), "fewer elements"), (dict(out=None), "output: null"),
+    (dict(out=0x10040), "overlaps codes"), (dict(out=0x30000), "overlaps tensor scale"),
+    (dict(m=dict(fmt=0)), "format"), (dict(m=dict(ld=0)), "multiple of 16"), (dict(m=dict(tensor_scale=None)), "needs a tensor scale"),
+])
+def test_dequantize_refusals(change, said):
+    a = dict(out=0x100000, dtype=A.F16, ld=64)
+    a.update({k: v for k, v in change.items() if k != "m"})
+    kw = change.get("m", {})
+    kw.setdefault("ld", 32)
+    m = matrix(**kw)
+    assert said in refused("b200c_mx_dequantize", C.byref(m.c), a["out"], a["dtype"], a["ld"])
+
+
+def test_null_descriptors_are_refused():
+    assert "null descriptor" in refused("b200c_mx_quantize", 0x1000, A.F16, 8, None, None, 0, 0)
+    assert "null descriptor" in refused("b200c_mx_dequantize", None, 0x1000, A.F16, 8)
+
+
+def test_oracle_rounds_to_the_nearest_code():
+    assert O.e2m1(np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 100.0, -0.3, -0.0])).tolist() == [0, 2, 2, 4, 4, 6, 6, 7, 9, 8]
+    assert O.e4m3(np.array([0.0, 448.0, 1.0, 2.0 ** -10, 3 * 2.0 ** -10, 17.0, 19.0])).tolist() == [0, 126, 56, 0, 2, 88, 90]
+
+
+# --------------------------------------------------------------------------- device side
+class Held:
+    """Buffers of a matrix on the device, each with canary bytes behind it."""
+
+    def __init__(self, fmt, rows, cols, layout, extra_ld=0, t=None):
+        self.fmt, self.rows, self.cols, self.layout = fmt, rows, cols, layout
+        pitch, _, nscale = mx.sizes(fmt, rows, cols, layout)
+        self.pitch, self.ld, self.nscale = pitch, pitch + extra_ld, nscale
+        self.codes = torch.full((rows * self.ld + 64,), CANARY, dtype=torch.uint8, device="cuda")
+        self.scales = torch.full((nscale + 64,), CANARY, dtype=torch.uint8, device="cuda")
+        self.tensor = torch.tensor([t if t is not None else -1.0, -1.0], device="cuda") if fmt == A.NVFP4 else None
+        self.m = mx.MxMatrix(fmt, rows, cols, self.codes.data_ptr(), self.scales.data_ptr(),
+                             None if self.tensor is None else self.tensor.data_ptr(), ld=self.ld, layout=layout)
+
+    def load(self, q, extra_noise=False):
+        """The oracle's codes and scales."""
+        self.codes[:self.rows * self.ld].view(self.rows, self.ld)[:, :self.pitch] = torch.from_numpy(O.pack(q["codes"])).cuda()
+        self.scales[:self.nscale] = torch.from_numpy(O.lay(q["scales"], self.layout)).cuda()
+        if self.tensor is not None:
+            self.tensor[0] = float(q["t"])
+        return self
+
+    def check(self, q):
+        """Every byte as the oracle has it, and nothing written that is not the matrix's."""
+        codes = self.codes.cpu().numpy()
+        body = codes[:self.rows * self.ld].reshape(self.rows, self.ld) if self.rows else codes[:0].reshape(0, max(self.ld, 1))
+        np.testing.assert_array_equal(body[:, :self.pitch], O.pack(q["codes"]))
+        assert (body[:, self.pitch:] == CANARY).all() and (codes[self.rows * self.ld:] == CANARY).all()
+        scales = self.scales.cpu().numpy()
+        np.testing.assert_array_equal(scales[:self.nscale], O.lay(q["scales"], self.layout))
+        assert (scales[self.nscale:] == CANARY).all()
+
+
+@pytest.fixture
+def dev(gpu):
+    """The backend on torch's current stream, so that tests order their work as torch does."""
+    gpu.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield gpu
+    torch.cuda.synchronize()
+    gpu.set_stream(None)
+
+
+def awkward(rows, cols, dtype, seed, special=True):
+    """Values over many magnitudes with ties, zeros of both signs, whole zero blocks, and (special) NaN, infinities,
+    the type's largest and smallest values."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((rows, cols)) * 2.0 ** rng.integers(-6, 6, (rows, 1))
+    ties = rng.integers(-24, 25, (rows, cols)) / 4.0
+    x = np.where(rng.random((rows, cols)) < 0.3, ties, x)
+    x[rng.random((rows, cols)) < 0.05] = -0.0
+    if cols > 40:
+        x[rows // 2, 7:40] = 0.0
+    t = torch.from_numpy(x).to(TYPES[dtype])
+    if special and rows > 2 and cols > 70:
+        info = torch.finfo(TYPES[dtype])
+        t[0, 3], t[1, 40], t[1, 70], t[2, 64] = float("nan"), float("inf"), -float("inf"), info.tiny
+        t[-1, :32] = info.smallest_normal / 4  # subnormal numbers only
+    return t
+
+
+def put(t, pad):
+    """On the device inside a wider buffer whose other columns are NaN; offset by `pad` elements from its start."""
+    rows, cols = t.shape
+    wide = torch.full((rows, cols + 2 * pad), float("nan"), dtype=t.dtype, device="cuda")
+    wide[:, pad:pad + cols] = t.cuda()
+    return wide[:, pad:pad + cols]
+
+
+SHAPES = [(1, 1), (1, 16), (1, 31), (3, 33), (5, 100), (129, 96), (130, 515), (2, 4100), (1, 11008), (700, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize(dev, fmt, dtype, rows, cols):
+    x = awkward(rows, cols, dtype, rows * 7 + cols)
+    q = O.quantize(x.double().numpy(), fmt)
+    for layout, pad, extra in ((A.MX_SCALES_ROWS, 0, 0), (A.MX_SCALES_TILED, 8, 16), (A.MX_SCALES_TILED, 3, 48)):
+        src = put(x, pad)
+        h = Held(fmt, rows, cols, layout, extra)
+        values = torch.full((rows, cols + pad), 7.0, dtype=x.dtype, device="cuda")
+        dev.mx_quantize(src.data_ptr(), dtype, src.stride(0), h.m, values=values.data_ptr(), values_ld=values.stride(0))
+        h.check(q)
+        # code * d has at most 24 + 2 bits: 32-bit rounding, then the type's
+        want = torch.from_numpy(q["values"].astype(np.float32)).to(x.dtype)
+        assert torch.equal(values[:, :cols].cpu().nan_to_num(nan=12345.0), want.nan_to_num(nan=12345.0))
+        assert (values[:, cols:] == 7.0).all()
+        if fmt == A.NVFP4:
+            assert h.tensor.tolist() == [float(q["t"]), float(q["top"])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1.0, 0.37, 2.0 ** -9, 3e-30, 1e30])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_quantize_with_a_given_tensor_scale(dev, dtype, t):
+    x = awkward(66, 200, dtype, 5)
+    q = O.quantize(x.double().numpy(), A.NVFP4, t=np.float32(t))
+    h = Held(A.NVFP4, 66, 200, A.MX_SCALES_TILED, t=t)
+    src = put(x, 0)
+    dev.mx_quantize(src.data_ptr(), dtype, src.stride(0), h.m, tensor_scale_given=True)
+    h.check(q)
+    assert h.tensor.tolist() == [float(np.float32(t)), -1.0]  # read, not written
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_extreme_magnitudes(dev, fmt):
+    """Every exponent of 32 bits, so that scales reach both ends of their range."""
+    rows = 254
+    e = np.arange(rows)[:, None] - 126.0
+    x = (np.random.default_rng(2).uniform(-1.99, 1.99, (rows, 64)) * 2.0 ** e).astype(np.float32)
+    for part in (x, x[:100], x[100:150]):
+        h = Held(fmt, len(part), 64, A.MX_SCALES_ROWS)
+        src = torch.from_numpy(part.copy()).cuda()
+        dev.mx_quantize(src.data_ptr(), A.F32, 64, h.m)
+        h.check(O.quantize(part, fmt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [0.0, -1.0, float("nan"), float("inf")])
+def test_given_scales_that_are_no_scales(dev, bad):
+    h = Held(A.NVFP4, 3, 32, A.MX_SCALES_ROWS, t=bad)
+    src = torch.ones(3, 32, device="cuda")
+    dev.mx_quantize(src.data_ptr(), A.F32, 32, h.m, tensor_scale_given=True)
+    assert (h.scales[:h.nscale] == 127).all() and (h.codes[:3 * 16] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_dequantize(dev, fmt, dtype, rows, cols):
+    rng = np.random.default_rng(rows + cols)
+    blocks = -(-cols // O.BLOCK[fmt])
+    # every scale byte that may be there, NaN among them
+    q = dict(codes=rng.integers(0, 16, (rows, cols)).astype(np.uint8),
+             scales=rng.integers(0, 256 if fmt == A.MXFP4 else 128, (rows, blocks)).astype(np.uint8), t=np.float32(0.3))
+    want = O.values_of(q["codes"], q["scales"], fmt, q["t"])
+    for layout, pad, extra in ((A.MX_SCALES_ROWS, 0, 16), (A.MX_SCALES_TILED, 8, 0), (A.MX_SCALES_TILED, 1, 0)):
+        h = Held(fmt, rows, cols, layout, extra).load(q)
+        out = torch.full((rows, cols + pad), 7.0, dtype=TYPES[dtype], device="cuda")
+        dev.mx_dequantize(h.m, out.data_ptr(), dtype, out.stride(0))
+        got = out[:, :cols].cpu()
+        # scale * t is rounded to 32 bits, code times that again, then the type rounds: with |w| the exact value,
+        # (2 * 2^-24 + eps / 2) |w| and a little for their product; half of the smallest step below the normal range
+        info = torch.finfo(TYPES[dtype])
+        with np.errstate(over="ignore"):
+            bound = np.abs(want) * (2 * 2.0 ** -24 + info.eps / 2) * 1.001 + info.smallest_normal * info.eps / 2 * 1.001
+        g = got.double().numpy()
+        nan = np.isnan(want)
+        assert (np.isnan(g) == nan).all()
+        over = np.abs(want) >= info.max * (1 + info.eps / 4)  # rounds to infinity
+        border = (np.abs(want) > info.max) & ~over
+        ok = np.abs(np.where(nan | over | border | np.isinf(g), 0, g - want)) <= bound
+        assert ok[~nan].all()
+        assert np.isinf(g[over & ~nan]).all() and not np.isinf(g[~over & ~border & ~nan]).any()
+        assert (out[:, cols:] == 7.0).all()
+
+
+@pytest.mark.gpu
+def test_empty_matrices(dev):
+    for rows, cols in ((0, 5), (5, 0), (0, 0)):
+        for fmt in FORMATS:
+            h = Held(fmt, rows, cols, A.MX_SCALES_TILED)
+            src = torch.ones(8, 8, device="cuda")
+            dev.mx_quantize(src.data_ptr(), A.F32, 8, h.m)
+            dev.mx_dequantize(h.m, src.data_ptr(), A.F32, 8)
+            assert (h.codes == CANARY).all() and (h.scales == CANARY).all() and (src == 1).all()
+            if fmt == A.NVFP4:
+                assert h.tensor.tolist() == [1.0, 0.0]
