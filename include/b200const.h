@@ -385,7 +385,12 @@ B200C_API int b200c_btc_compress_inplace_end(b200c_ctx* ctx, int ticket, size_t*
  * every scale becomes NaN) and nothing is written there.  `values` (may be NULL): what the codes stand
  * for, in the type of src, values_ld elements between rows.
  *
- * b200c_mx_dequantize: what the codes of `m` stand for -> out (f16, bf16 or f32, rounded from 32 bits).   */
+ * b200c_mx_dequantize: what the codes of `m` stand for -> out (f16, bf16 or f32, rounded from 32 bits).
+ *
+ * b200c_mx_matmul: out[i][j] = sum_k A[i][k] B[j][k] for A = a [rows x cols], B = b [rows x cols of a], both of
+ * one format and with tiled scales; sums in 32 bits, times both t; out f16, bf16 or f32, out_ld elements
+ * between rows.  A row of A or B with a NaN scale makes the outputs it takes part in NaN.  One result is
+ * the same bytes on every run.                                                              */
 #define B200C_MXFP4 1
 #define B200C_NVFP4 2
 #define B200C_MX_SCALES_ROWS 0
@@ -405,6 +410,8 @@ B200C_API int b200c_mx_sizes(int32_t format, int32_t scale_layout, int64_t rows,
 B200C_API int b200c_mx_quantize(b200c_ctx* ctx, const void* src, int32_t src_dtype, int64_t src_ld,
                                 const b200c_mx_matrix* out, void* values, int64_t values_ld, int flags);
 B200C_API int b200c_mx_dequantize(b200c_ctx* ctx, const b200c_mx_matrix* m, void* out, int32_t out_dtype, int64_t out_ld);
+B200C_API int b200c_mx_matmul(b200c_ctx* ctx, const b200c_mx_matrix* a, const b200c_mx_matrix* b, void* out, int32_t out_dtype,
+                              int64_t out_ld);
 
 /* ---- splat detection -------------------------------------------------------------
  * "All elements equal" test of a raw buffer: detectSplatElementWise, which the reference runs when

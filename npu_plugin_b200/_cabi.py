@@ -180,6 +180,7 @@ SYMBOLS = {
     "b200c_mx_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, _P(b200c_mx_matrix), C.c_void_p, C.c_int64,
                                     C.c_int]),
     "b200c_mx_dequantize": (C.c_int, [C.c_void_p, _P(b200c_mx_matrix), C.c_void_p, C.c_int32, C.c_int64]),
+    "b200c_mx_matmul": (C.c_int, [C.c_void_p, _P(b200c_mx_matrix), _P(b200c_mx_matrix), C.c_void_p, C.c_int32, C.c_int64]),
     "b200c_detect_splat": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int, _P(C.c_int)]),
     "b200c_digest64_batch": (C.c_int, [C.c_void_p, C.c_int, _P(C.c_void_p), _P(C.c_size_t), _P(C.c_uint64)]),
     "b200c_ipc_export": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, _P(b200c_ipc_handle)]),

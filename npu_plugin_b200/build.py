@@ -12,7 +12,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_obj")
 SOURCES = ["api.cu", "plan.cu", "fold_kernels.cu", "rowquant_kernels.cu", "tile_kernels.cu", "dequant_kernels.cu",
            "sparsity_kernels.cu", "codec_kernels.cu", "synth_kernels.cu", "probe_kernels.cu", "exchange_kernels.cu",
-           "mx_kernels.cu", "mx.cpp", "infer.cpp"]
+           "mx_kernels.cu", "mx_matmul.cu", "mx.cpp", "infer.cpp"]
 HEADERS = ["ctype.h", "view.h", "runtime.h", "plan.h", "codec.h", "mx.h", os.path.join("..", "..", "include", "b200const.h")]
 LIB = os.path.join(CSRC, "libb200const.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

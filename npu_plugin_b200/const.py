@@ -561,6 +561,12 @@ class CudaBackend:
         if rc:
             raise_for(rc, self._err())
 
+    def mx_matmul(self, a, b, out, dtype, out_ld):
+        """out = a b^T of two matrices with tiled scales (out f16/bf16/f32, out_ld elements between rows)."""
+        rc = self.lib.b200c_mx_matmul(self.ctx, C.byref(a.c), C.byref(b.c), out, dtype, out_ld)
+        if rc:
+            raise_for(rc, self._err())
+
     def synth_fill(self, dev_ptr, count, dtype, dist, p0, p1, seed, stream_id):
         raise_for(self.lib.b200c_synth_fill(self.ctx, dev_ptr, int(count), dtype, dist, p0, p1, seed, stream_id), self._err())
 

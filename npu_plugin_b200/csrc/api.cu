@@ -140,6 +140,8 @@ static const char* errText(int code) {
         return "Sparsify: more non-sparse elements than numActualElements allows";
     case E_CODEC:
         return "codec: malformed stream or output capacity exceeded";
+    case E_STALLED:
+        return "a wait inside a kernel gave up: its results are not valid";
     default:
         return "unknown device-side error";
     }
@@ -1042,6 +1044,17 @@ int b200c_mx_dequantize(b200c_ctx* h, const b200c_mx_matrix* m, void* out, int32
         Context* ctx = reinterpret_cast<Context*>(h);
         MxScope scope(ctx);
         launchMxDequantize(ctx, *m, out, out_dtype, out_ld);
+    });
+}
+
+int b200c_mx_matmul(b200c_ctx* h, const b200c_mx_matrix* a, const b200c_mx_matrix* b, void* out, int32_t out_dtype,
+                    int64_t out_ld) {
+    return guarded([&] {
+        mxCheckMatmul(a, b, out, out_dtype, out_ld);
+        if (!h) throw BadArg("null context");
+        Context* ctx = reinterpret_cast<Context*>(h);
+        MxScope scope(ctx);
+        launchMxMatmul(ctx, *a, *b, out, out_dtype, out_ld);
     });
 }
 

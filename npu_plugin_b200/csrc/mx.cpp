@@ -122,4 +122,19 @@ void mxCheckDequantize(const b200c_mx_matrix* m, const void* out, int dtype, int
     checkApart(dst, in.tensor);
 }
 
+void mxCheckMatmul(const b200c_mx_matrix* a, const b200c_mx_matrix* b, const void* out, int dtype, int64_t outLd) {
+    const MatrixRanges ra = checkMatrix("left matrix", a), rb = checkMatrix("right matrix", b);
+    if (a->format != b->format) throw BadArg("the two matrices have different formats");
+    if (a->cols != b->cols) throw BadArg("the two matrices have different numbers of columns");
+    if (a->scale_layout != B200C_MX_SCALES_TILED || b->scale_layout != B200C_MX_SCALES_TILED) {
+        throw BadArg("the product reads tiled scales");
+    }
+    const Range dst = checkDense("output", out, dtype, a->rows, b->rows, outLd);
+    for (const MatrixRanges* m : {&ra, &rb}) {
+        checkApart(dst, m->codes);
+        checkApart(dst, m->scales);
+        checkApart(dst, m->tensor);
+    }
+}
+
 }  // namespace b200c

@@ -1,5 +1,5 @@
 // Block-scaled 4-bit matrices: descriptors, sizes and the checks of their arguments (mx.cpp), and the
-// launchers of the kernels (mx_kernels.cu).  Formats and storage: include/b200const.h.
+// launchers of the kernels (mx_kernels.cu, mx_matmul.cu).  Formats and storage: include/b200const.h.
 #pragma once
 
 #include "../../include/b200const.h"
@@ -29,9 +29,11 @@ void mxCheckShape(int format, int layout, int64_t rows, int64_t cols);
 void mxCheckQuantize(const void* src, int dtype, int64_t srcLd, const b200c_mx_matrix* out, const void* values,
                      int64_t valuesLd, int flags);
 void mxCheckDequantize(const b200c_mx_matrix* m, const void* out, int dtype, int64_t outLd);
+void mxCheckMatmul(const b200c_mx_matrix* a, const b200c_mx_matrix* b, const void* out, int dtype, int64_t outLd);
 
 void launchMxQuantize(Context* ctx, const void* src, int dtype, int64_t srcLd, const b200c_mx_matrix& out, void* values,
                       int64_t valuesLd, bool scaleGiven);
 void launchMxDequantize(Context* ctx, const b200c_mx_matrix& m, void* out, int dtype, int64_t outLd);
+void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matrix& b, void* out, int dtype, int64_t outLd);
 
 }  // namespace b200c

@@ -65,7 +65,8 @@ enum FoldErr : int {
     E_CAST_INEXACT = 2,  // int -> float or double -> float does not round-trip
     E_OOB = 3,           // out-of-bound access checks of the reference
     E_SPARSE_OVERFLOW = 4,
-    E_CODEC = 5
+    E_CODEC = 5,
+    E_STALLED = 6
 };
 
 constexpr int kMaxDims = 8;

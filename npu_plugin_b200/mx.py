@@ -1,6 +1,6 @@
 """Block-scaled 4-bit matrices for Python callers: descriptors and sizes.  The arithmetic is in
-libb200const.so (b200c_mx_quantize, b200c_mx_dequantize; formats and storage in include/b200const.h) and is called
-through the backend: CudaBackend.mx_quantize / mx_dequantize.  No counterpart in the reference, whose
+libb200const.so (b200c_mx_quantize, b200c_mx_dequantize, b200c_mx_matmul; formats and storage in include/b200const.h) and is called
+through the backend: CudaBackend.mx_quantize / mx_dequantize / mx_matmul.  No counterpart in the reference, whose
 narrowest weights are int4 with one scale per channel."""
 import ctypes as C
 

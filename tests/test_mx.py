@@ -261,3 +261,158 @@ def test_empty_matrices(dev):
             assert (h.codes == CANARY).all() and (h.scales == CANARY).all() and (src == 1).all()
             if fmt == A.NVFP4:
                 assert h.tensor.tolist() == [1.0, 0.0]
+
+
+# --------------------------------------------------------------------------- product
+@pytest.mark.parametrize("change,said", [
+    (dict(), "null context"), (dict(dtype=A.I8), "element type"), (dict(ld=63), "fewer elements"), (dict(out=None), "output: null"),
+    (dict(out=0x10000), "overlaps codes"), (dict(out=0x51000), "overlaps scales"), (dict(a=dict(fmt=A.MXFP4)), "different formats"),
+    (dict(a=dict(cols=96, ld=48)), "different numbers"), (dict(a=dict(layout=A.MX_SCALES_ROWS)), "tiled scales"),
+    (dict(b=dict(layout=A.MX_SCALES_ROWS)), "tiled scales"), (dict(b=dict(tensor_scale=None)), "needs a tensor scale"),
+    (dict(a=dict(codes=0x10001)), "16-byte"), (dict(a=dict(ld=24)), "multiple of 16"),
+])
+def test_matmul_refusals(change, said):
+    a = matrix(**dict(dict(ld=32), **change.get("a", {})))
+    b = matrix(**dict(dict(ld=32, codes=0x50000, scales=0x51000, tensor_scale=0x52000), **change.get("b", {})))
+    args = dict(dict(out=0x100000, dtype=A.F32, ld=64), **{k: v for k, v in change.items() if k not in "ab"})
+    assert said in refused("b200c_mx_matmul", C.byref(a.c), C.byref(b.c), args["out"], args["dtype"], args["ld"])
+    assert "null descriptor" in refused("b200c_mx_matmul", None, C.byref(b.c), args["out"], args["dtype"], args["ld"])
+
+
+def random_held(fmt, rows, cols, seed, spread=4, extra_ld=0):
+    """A matrix of random codes and scales in the product's layout: scales over 2^(2 * spread)."""
+    rng = np.random.default_rng(seed)
+    blocks = -(-cols // O.BLOCK[fmt])
+    mid = 127 if fmt == A.MXFP4 else 56
+    step = 1 if fmt == A.MXFP4 else 8
+    scales = rng.integers(mid - spread * step, mid + spread * step + 1, (rows, blocks)).astype(np.uint8)
+    q = dict(codes=rng.integers(0, 16, (rows, cols)).astype(np.uint8), scales=scales, t=np.float32(2.0 ** -rng.integers(0, 9)))
+    return Held(fmt, rows, cols, A.MX_SCALES_TILED, extra_ld).load(q), O.values_of(q["codes"], q["scales"], fmt, q["t"])
+
+
+def check_product(got, va, vb, dtype):
+    want = va @ vb.T
+    size = np.abs(va) @ np.abs(vb).T
+    # products are exact; a step of 64 adds to the 32-bit sum with at most one unit in the last place lost, and the
+    # sums' scale once more; then the type rounds, half a step of its subnormal range at least
+    steps = -(-va.shape[1] // 64) + 2
+    info = torch.finfo(TYPES[dtype])
+    bound = steps * 2.0 ** -23 * size + np.abs(want) * info.eps / 2 * (1 + 2.0 ** -10) + info.smallest_normal * info.eps / 2
+    over = np.abs(want) > info.max
+    assert not np.isnan(got).any()
+    far = np.where(over, 0, np.abs(got - want)) - bound
+    assert (far <= 0).all(), (far.max(), np.unravel_index(far.argmax(), far.shape))
+
+
+PRODUCTS = [(1, 1, 1), (1, 128, 32), (3, 5, 16), (16, 130, 100), (17, 300, 257), (64, 64, 64), (65, 1000, 515), (128, 129, 300),
+            (129, 128, 1003), (200, 300, 4100), (300, 20, 777), (257, 513, 2048), (1, 1000, 11008), (130, 1, 96)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_matmul(dev, fmt, m, n, k):
+    a, va = random_held(fmt, m, k, m + k, extra_ld=16 if n % 2 else 0)
+    b, vb = random_held(fmt, n, k, n + 3 * k)
+    for dtype, pad in ((A.F32, 0), (A.BF16, 8), (A.F16, 3)):
+        out = torch.full((m, n + pad), 7.0, dtype=TYPES[dtype], device="cuda")
+        dev.mx_matmul(a.m, b.m, out.data_ptr(), dtype, out.stride(0))
+        dev.synchronize()
+        got = out.double().cpu().numpy()
+        check_product(got[:, :n], va, vb, dtype)
+        assert (got[:, n:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(16, 256, 1024), (300, 700, 2048)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_matmul_is_exact_where_sums_are(dev, fmt, m, n, k):
+    """Scales of one: every product is a multiple of 1/4 below 36, so sums of up to 2^17 of them fit 24 bits."""
+    rng = np.random.default_rng(k)
+    one = 127 if fmt == A.MXFP4 else 56
+    sides = []
+    for rows in (m, n):
+        q = dict(codes=rng.integers(0, 16, (rows, k)).astype(np.uint8),
+                 scales=np.full((rows, k // O.BLOCK[fmt]), one, np.uint8), t=np.float32(1))
+        sides.append((Held(fmt, rows, k, A.MX_SCALES_TILED).load(q), O.decode(q["codes"])))
+    (a, va), (b, vb) = sides
+    out = torch.empty(m, n, device="cuda")
+    dev.mx_matmul(a.m, b.m, out.data_ptr(), A.F32, n)
+    np.testing.assert_array_equal(out.double().cpu().numpy(), va @ vb.T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_matmul_keeps_nan_to_its_rows(dev, fmt):
+    """A NaN scale in one row of each side; the scales that fill up the tiles are NaN too, and must not matter."""
+    m, n, k = 20, 150, 200
+    a, va = random_held(fmt, m, k, 1)
+    b, vb = random_held(fmt, n, k, 2)
+    nan = 255 if fmt == A.MXFP4 else 127
+    want = va @ vb.T
+    for h, rows in ((a, m), (b, n)):
+        mark = np.zeros((-(-rows // 128) * 128, -(-k // O.BLOCK[fmt])), np.uint8)
+        mark[rows:] = 1  # rows behind the last
+        mark[7, 3] = 1
+        laid = torch.from_numpy(O.lay(mark, 1)).cuda().bool()
+        h.scales[:h.nscale][laid] = nan
+    out = torch.empty(m, n, device="cuda")
+    dev.mx_matmul(a.m, b.m, out.data_ptr(), A.F32, n)
+    got = out.double().cpu().numpy()
+    bad = np.zeros((m, n), bool)
+    bad[7], bad[:, 7] = True, True
+    assert np.isnan(got[bad]).all()
+    assert np.isfinite(got[~bad]).all() and np.allclose(got[~bad], want[~bad], rtol=1e-4, atol=1e-4 * np.abs(want).max())
+
+
+@pytest.mark.gpu
+def test_matmul_of_nothing(dev):
+    for fmt in FORMATS:
+        a, b = Held(fmt, 3, 0, A.MX_SCALES_TILED), Held(fmt, 5, 0, A.MX_SCALES_TILED)
+        out = torch.full((3, 6), 7.0, device="cuda")
+        dev.mx_matmul(a.m, b.m, out.data_ptr(), A.F32, 6)
+        assert (out[:, :5] == 0).all() and (out[:, 5] == 7).all()
+        e, f = Held(fmt, 0, 64, A.MX_SCALES_TILED), Held(fmt, 5, 64, A.MX_SCALES_TILED)
+        dev.mx_matmul(e.m, f.m, out.data_ptr(), A.F32, 6)
+        dev.mx_matmul(f.m, e.m, out.data_ptr(), A.F32, 6)
+        assert (out[:, 5] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantise_then_multiply(dev, fmt):
+    """A linear layer as a program runs it: weights once, activations and the product every time, also captured."""
+    m, n, k = 5, 200, 300
+    rng = np.random.default_rng(9)
+    w = torch.from_numpy(rng.standard_normal((n, k)).astype(np.float32)).half()
+    qw = O.quantize(w.double().numpy(), fmt)
+    hw = Held(fmt, n, k, A.MX_SCALES_TILED)
+    dw = w.cuda()
+    dev.mx_quantize(dw.data_ptr(), A.F16, k, hw.m)
+    hx = Held(fmt, m, k, A.MX_SCALES_TILED)
+    dx = torch.zeros(m, k, dtype=torch.half, device="cuda")
+    out = torch.empty(m, n, dtype=torch.half, device="cuda")
+
+    def step():
+        dev.mx_quantize(dx.data_ptr(), A.F16, k, hx.m)
+        dev.mx_matmul(hx.m, hw.m, out.data_ptr(), A.F16, n)
+
+    def check(x):
+        qx = O.quantize(x.double().numpy(), fmt)
+        check_product(out.double().cpu().numpy(), qx["values"], qw["values"], A.F16)
+
+    xs = [torch.from_numpy(rng.standard_normal((m, k)) * s).half() for s in (1.0, 30.0)]
+    dx.copy_(xs[0])
+    step()
+    check(xs[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        dev.set_stream(torch.cuda.current_stream().cuda_stream)
+        step()
+    dev.set_stream(torch.cuda.current_stream().cuda_stream)
+    for x in (xs[1], xs[0]):
+        dx.copy_(x)
+        graph.replay()
+        check(x)
