@@ -14,6 +14,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <string>
+#include <type_traits>
 
 namespace b200c {
 
@@ -28,7 +30,8 @@ struct MxMatmulParams {
     long long chunks;      // tiles of 4 blocks along k: 512 bytes of scales each, per 128 rows
     int scaleTilesQ;       // tiles of 128 rows that the Q side's scales have
     int ktiles;
-    int tilesQ;
+    int tilesP, tilesQ;
+    int split;             // CTAs that share a tile's k
     void* out;
     long long ld;
     int outTag;            // T_F16, T_BF16, T_F32
@@ -41,20 +44,37 @@ constexpr int kTileK = 256;      // elements of k per stage: 128 bytes of codes,
 constexpr int kStepK = 64;       // elements of k per tcgen05.mma
 constexpr int kThreads = 192;    // warps 0-3: epilogue, 4: loads, 5: mma
 
+// One CTA, 128 rows of P by BN rows of Q.
 template <int BN, bool NV>
 struct Tile {
     static constexpr int chunksPerTile = NV ? 4 : 2;  // 512-byte tiles of scales per stage and 128 rows
-    static constexpr int rowTilesQ = (BN + 127) / 128;
     static constexpr int bytesP = 128 * 128;
     static constexpr int bytesQ = BN * 128;
-    static constexpr int scaleBytesP = chunksPerTile * 512;
-    static constexpr int scaleBytesQ = scaleBytesP * rowTilesQ;
-    static constexpr int stageBytes = (bytesP + bytesQ + scaleBytesP + scaleBytesQ + 1023) / 1024 * 1024;
-    static constexpr int stages = 4;
-    static constexpr int smemBytes = 1024 /* barriers */ + 1024 /* alignment */ + stages * stageBytes;
-    static constexpr int scaleCols = chunksPerTile * 4 * (1 + rowTilesQ);  // tensor memory columns of a stage's scales
-    static constexpr int needCols = BN + 2 * scaleCols;
-    static constexpr int cols = needCols <= 32 ? 32 : needCols <= 64 ? 64 : needCols <= 128 ? 128 : needCols <= 256 ? 256 : 512;
+    static constexpr int scaleBytes = chunksPerTile * 512;  // of each side: no tile of Q crosses 128 rows
+    static constexpr int stageBytes = (bytesP + bytesQ + 2 * scaleBytes + 1023) / 1024 * 1024;
+    static constexpr int stages = BN <= 32 ? 4 : 3;         // two CTAs fit an SM
+    static constexpr int smemBytes = 1024 /* alignment */ + stages * stageBytes;
+    static constexpr int scaleCols = 2 * chunksPerTile * 4;  // tensor memory columns of a stage's scales
+    static constexpr int scaleBufs = 2;
+    static constexpr int needCols = BN + scaleBufs * scaleCols;
+    static constexpr int cols = needCols <= 64 ? 64 : needCols <= 128 ? 128 : 256;
+    static_assert(stages * stageBytes >= 128 * BN * 4, "the partial sums of a split tile use the stages' memory");
+};
+
+// Two CTAs, 256 rows of P by 256 rows of Q: each CTA holds 128 rows of both sides and the sums of its 128
+// rows of P.  Tensor memory: the sums of alternate tiles lie in columns 0..255 and 160..415, the scales behind.
+template <bool NV>
+struct PairTile {
+    static constexpr int chunksPerTile = NV ? 4 : 2;
+    static constexpr int bytesSide = 128 * 128;
+    static constexpr int scaleBytes = chunksPerTile * 512;  // of 128 rows
+    static constexpr int stageBytes = (2 * bytesSide + 3 * scaleBytes + 1023) / 1024 * 1024;
+    static constexpr int stages = NV ? 5 : 6;
+    static constexpr int smemBytes = 1024 + stages * stageBytes;
+    static constexpr int accStep = 160, scaleCol = 416;
+    static constexpr int scaleCols = 3 * chunksPerTile * 4;
+    static constexpr int scaleBufs = 96 / scaleCols;
+    static constexpr int cols = 512;
 };
 
 __device__ __forceinline__ unsigned int smemAddr(const void* p) {
@@ -91,6 +111,36 @@ __device__ __forceinline__ bool barWait(unsigned int bar, unsigned int parity, v
     return barWaitSlow(bar, parity, stalled);
 }
 
+// One thread of the warp, the same one every time and known to the compiler as such: the operands of
+// what it issues stay in uniform registers.  Issued from a lane picked by its number the same
+// instructions took 1.9 times as long (0.91 instead of 0.48 us per 256 elements of k of a 128 x 256 tile).
+__device__ __forceinline__ bool electOne() {
+    unsigned int one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+__device__ __forceinline__ unsigned int clusterRank() {
+    unsigned int r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void clusterSync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned int addrIn(unsigned int addr, unsigned int rank) {
+    unsigned int r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void expectBytes(unsigned int bar, unsigned int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void drain(unsigned int bar, unsigned int parity) {
+    const long long start = clock64();
+    while (!barTry(bar, parity) && clock64() - start < 4000000000ll) {
+    }
+}
+
 __device__ __forceinline__ void loadTile(unsigned int dst, const CUtensorMap* map, int x, int y, unsigned int bar) {
     asm volatile(
             "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -118,34 +168,73 @@ __device__ __forceinline__ void copyScales(unsigned int tmem, unsigned long long
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 
-template <bool NV>
+// The same loads for one CTA of a pair, counted at a barrier of either.
+__device__ __forceinline__ void loadTilePair(unsigned int dst, const CUtensorMap* map, int x, int y, unsigned int bar) {
+    asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+__device__ __forceinline__ void loadScalesPair(unsigned int dst, const CUtensorMap* map, int chunk, int tile, unsigned int bar) {
+    asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                    dst),
+            "l"(map), "r"(0), "r"(chunk), "r"(tile), "r"(bar)
+            : "memory");
+}
+__device__ __forceinline__ void copyScalesPair(unsigned int tmem, unsigned long long desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+#define B2_MX_MMA(group, kind)                                                                                              \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::" group ".kind::" kind                  \
+                 " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                                                         \
+                 "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate)                                      \
+                 : "memory")
+template <bool NV, bool PAIR>
 __device__ __forceinline__ void mma(unsigned int d, unsigned long long a, unsigned long long b, unsigned int idesc,
                                     unsigned int scaleA, unsigned int scaleB, unsigned int accumulate) {
-    if (NV) {
-        asm volatile(
-                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-                "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate)
-                : "memory");
+    if (NV && PAIR) {
+        B2_MX_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    } else if (NV) {
+        B2_MX_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    } else if (PAIR) {
+        B2_MX_MMA("2", "mxf4.block_scale.scale_vec::2X");
     } else {
-        asm volatile(
-                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-                "l"(a), "l"(b), "r"(idesc), "r"(scaleA), "r"(scaleB), "r"(accumulate)
-                : "memory");
+        B2_MX_MMA("1", "mxf4.block_scale.scale_vec::2X");
     }
 }
-// arrives at `bar` once everything issued so far by this thread to the tensor core is done
+#undef B2_MX_MMA
+// arrives at `bar` (of both CTAs of a pair) once everything issued so far by this thread to the tensor core is done
 __device__ __forceinline__ void mmaCommit(unsigned int bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void mmaCommitPair(unsigned int bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<unsigned short>(3))
+                 : "memory");
+}
 
-// Instruction descriptor: e2m1 x e2m1, 128 x BN; the scales' type in bit 23 (1: e8m0); which pair of a word's
+// Instruction descriptor: e2m1 x e2m1, M x N; the scales' type in bit 23 (1: e8m0); which pair of a word's
 // four scale bytes is meant in bits 29 (A) and 4 (B).
-template <int BN, bool NV>
+template <int M, int N, bool NV>
 __device__ __forceinline__ unsigned int instruction(int pair) {
-    return (1u << 7) | (1u << 10) | (static_cast<unsigned int>(BN >> 3) << 17) | (NV ? 0u : 1u << 23) | (1u << 27) |
-           (static_cast<unsigned int>(pair) << 29) | (static_cast<unsigned int>(pair) << 4);
+    return (1u << 7) | (1u << 10) | (static_cast<unsigned int>(N >> 3) << 17) | (NV ? 0u : 1u << 23) |
+           (static_cast<unsigned int>(M >> 7) << 27) | (static_cast<unsigned int>(pair) << 29) | (static_cast<unsigned int>(pair) << 4);
+}
+
+// The products of one stage: up to four steps of 64 elements of k.  A word of four scales reaches over one step
+// (nvfp4) or two (mxfp4); `wordsQ` columns of tensor memory lie between the words of Q.
+template <int M, int N, bool NV, bool PAIR>
+__device__ __forceinline__ void mmaStage(unsigned int acc, unsigned long long dp, unsigned long long dq, unsigned int colP,
+                                         unsigned int colQ, int wordsQ, int steps, bool first) {
+#pragma unroll
+    for (int i = 0; i < kTileK / kStepK; ++i) {
+        if (i < steps) {
+            const int c = NV ? i : i >> 1, pair = NV ? 0 : (i & 1) * 2;
+            mma<NV, PAIR>(acc, dp + i * 2, dq + i * 2, instruction<M, N, NV>(pair), colP + c * 4, colQ + c * wordsQ, !(first && i == 0));
+        }
+    }
 }
 
 __device__ __forceinline__ void readColumns(unsigned int addr, float v[32]) {
@@ -206,10 +295,10 @@ __device__ __forceinline__ void storeColumns(const MxMatmulParams& g, long long 
         return;
     }
     T* row = out + p * g.ld + q0;
-    constexpr int per = 16 / sizeof(T);
+    constexpr int per = N < static_cast<int>(16 / sizeof(T)) ? N : 16 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < N; i += per) {
-        if (g.wide && i + per <= left) {
+        if (N >= static_cast<int>(16 / sizeof(T)) && g.wide && i + per <= left) {
             alignas(16) T t[per];
 #pragma unroll
             for (int j = 0; j < per; ++j) t[j] = toOut<T>(v[i + j]);
@@ -239,6 +328,25 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
     }
 }
 
+// The tile's sums lie in `split` CTAs' shared memory as [BN][128]; this CTA adds up its share of the columns, in
+// the order of the ranks.
+template <class T, int BN>
+__device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int row, long long p, long long q0,
+                                            float alpha) {
+    const int c0 = static_cast<int>(rank) * BN / g.split, c1 = (static_cast<int>(rank) + 1) * BN / g.split;
+    for (int c = c0; c < c1; ++c) {
+        if (q0 + c >= g.rowsQ) break;
+        float v = 0.f;
+        for (int r = 0; r < g.split; ++r) {
+            float w;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(addrIn(sums + (c * 128 + row) * 4, r)) : "memory");
+            v = v + w;
+        }
+        const float one[1] = {v * alpha};
+        storeColumns<T, 1>(g, p, q0 + c, one);
+    }
+}
+
 template <int BN, bool NV>
 __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                                                            const __grid_constant__ MxMatmulParams g) {
@@ -250,9 +358,13 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     volatile int* stalled = &stalledWord;
     const unsigned int stage0 = (smemAddr(raw) + 1023u) & ~1023u;
     const unsigned int full = smemAddr(bars), empty = full + 8 * S::stages, done = empty + 8 * S::stages;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long p0 = static_cast<long long>(blockIdx.x / g.tilesQ) * 128;
-    const long long q0 = static_cast<long long>(blockIdx.x % g.tilesQ) * BN;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const unsigned int rank = g.split > 1 ? clusterRank() : 0;
+    const int tile = blockIdx.x / g.split;
+    const long long p0 = static_cast<long long>(tile / g.tilesQ) * 128;
+    const long long q0 = static_cast<long long>(tile % g.tilesQ) * BN;
+    const int k0 = static_cast<int>(static_cast<long long>(g.ktiles) * rank / g.split);
+    const int n = static_cast<int>(static_cast<long long>(g.ktiles) * (rank + 1) / g.split) - k0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::stages; ++s) {
@@ -272,87 +384,282 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned int acc = tmemBase, scaleCol = tmemBase + BN;
 
-    if (warp == 4 && lane == 0) {
-        const int scaleTileP = static_cast<int>(p0 / 128), scaleTileQ = static_cast<int>(q0 / 128);
-        const int tilesQ = min(S::rowTilesQ, g.scaleTilesQ - scaleTileQ);  // rows behind the last tile have no scales
-        int issued = 0;
-        for (int kt = 0; kt < g.ktiles; ++kt) {
-            const int s = kt % S::stages;
-            if (kt >= S::stages && !barWait(empty + 8 * s, ((kt / S::stages) & 1) ^ 1, stalled)) break;
-            const unsigned int at = stage0 + s * S::stageBytes, bar = full + 8 * s;
-            const long long chunk = static_cast<long long>(kt) * S::chunksPerTile;
-            const unsigned int scaleBytes = static_cast<unsigned int>(min(static_cast<long long>(S::chunksPerTile), g.chunks - chunk)) * 512u;
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
-                         "r"(S::bytesP + S::bytesQ + scaleBytes * (1 + tilesQ))
-                         : "memory");
-            loadTile(at, &mapP, kt * 128, static_cast<int>(p0), bar);
-            loadTile(at + S::bytesP, &mapQ, kt * 128, static_cast<int>(q0), bar);
-            const unsigned int sp = at + S::bytesP + S::bytesQ;
-            loadBytes(sp, g.scalesP + (scaleTileP * g.chunks + chunk) * 512, scaleBytes, bar);
-            for (int i = 0; i < tilesQ; ++i) {
-                loadBytes(sp + S::scaleBytesP * (1 + i), g.scalesQ + ((scaleTileQ + i) * g.chunks + chunk) * 512, scaleBytes, bar);
+    if (warp == 4) {
+        const long long scaleTileP = p0 / 128, scaleTileQ = q0 / 128;
+        int s = 0, phase = 1, issued = 0;
+        for (; issued < n; ++issued) {
+            if (!__all_sync(0xFFFFFFFFu, issued < S::stages || barWait(empty + 8 * s, phase, stalled))) break;
+            if (electOne()) {
+                const int kt = k0 + issued;
+                const unsigned int at = stage0 + s * S::stageBytes, bar = full + 8 * s;
+                const long long chunk = static_cast<long long>(kt) * S::chunksPerTile;
+                const unsigned int scaleBytes = static_cast<unsigned int>(min(static_cast<long long>(S::chunksPerTile), g.chunks - chunk)) * 512u;
+                expectBytes(bar, S::bytesP + S::bytesQ + 2 * scaleBytes);
+                loadTile(at, &mapP, kt * 128, static_cast<int>(p0), bar);
+                loadTile(at + S::bytesP, &mapQ, kt * 128, static_cast<int>(q0), bar);
+                const unsigned int sp = at + S::bytesP + S::bytesQ;
+                loadBytes(sp, g.scalesP + (scaleTileP * g.chunks + chunk) * 512, scaleBytes, bar);
+                loadBytes(sp + S::scaleBytes, g.scalesQ + (scaleTileQ * g.chunks + chunk) * 512, scaleBytes, bar);
             }
-            issued = kt + 1;
+            __syncwarp();
+            if (++s == S::stages) s = 0, phase ^= 1;
         }
         // a wait that gave up leaves copies in flight: they write this CTA's memory, so it stays until they have
         if (*stalled) {
-            for (int kt = max(0, issued - S::stages); kt < issued; ++kt) {
-                const long long start = clock64();
-                while (!barTry(full + 8 * (kt % S::stages), (kt / S::stages) & 1) && clock64() - start < 4000000000ll) {
-                }
-            }
+            for (int i = max(0, issued - S::stages); i < issued; ++i) drain(full + 8 * (i % S::stages), (i / S::stages) & 1);
         }
-    } else if (warp == 5 && lane == 0) {
-        bool ok = true;
-        for (int kt = 0; kt < g.ktiles; ++kt) {
-            const int s = kt % S::stages;
-            ok = barWait(full + 8 * s, (kt / S::stages) & 1, stalled);
-            if (!ok) break;
+    } else if (warp == 5) {
+        const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesP);
+        const unsigned long long ds0 = scaleDesc(stage0 + S::bytesP + S::bytesQ);
+        // rows of a Q tile that starts inside 128 rows: the scales of 32 rows are one column of a word's four
+        const unsigned int shiftQ = static_cast<unsigned int>(q0 % 128) / 32;
+        int s = 0, phase = 0;
+        for (int i = 0; i < n; ++i) {
+            bool ok = barWait(full + 8 * s, phase, stalled);
+            // the scales' columns are free once the products that read them are done: nothing else orders a copy behind them
+            if (i >= S::scaleBufs) ok = ok && barWait(empty + 8 * ((i - S::scaleBufs) % S::stages), ((i - S::scaleBufs) / S::stages) & 1, stalled);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned int at = stage0 + s * S::stageBytes;
-            const unsigned int sp = at + S::bytesP + S::bytesQ;
-            const unsigned int colP = scaleCol + (kt & 1) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
-            const long long leftK = g.k - static_cast<long long>(kt) * kTileK;
-            const int steps = static_cast<int>(min(static_cast<long long>(kTileK / kStepK), (leftK + kStepK - 1) / kStepK));
-            const int chunks = static_cast<int>(min(static_cast<long long>(S::chunksPerTile), g.chunks - static_cast<long long>(kt) * S::chunksPerTile));
-            for (int c = 0; c < chunks; ++c) {
-                copyScales(colP + c * 4, scaleDesc(sp + c * 512));
-                for (int i = 0; i < S::rowTilesQ; ++i) {
-                    copyScales(colQ + (c * S::rowTilesQ + i) * 4, scaleDesc(sp + S::scaleBytesP * (1 + i) + c * 512));
+            if (electOne()) {
+                const int kt = k0 + i;
+                const unsigned int colP = scaleCol + (i % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
+                const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
+                const bool whole = kt + 1 < g.ktiles;
+                const int chunks = whole ? S::chunksPerTile : static_cast<int>(g.chunks - static_cast<long long>(kt) * S::chunksPerTile);
+                const int steps = whole ? kTileK / kStepK : static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+#pragma unroll
+                for (int c = 0; c < S::chunksPerTile; ++c) {
+                    if (c < chunks) {
+                        copyScales(colP + c * 4, ds0 + off + c * 32);
+                        copyScales(colQ + c * 4, ds0 + off + S::scaleBytes / 16 + c * 32);
+                    }
                 }
+                mmaStage<128, BN, NV, false>(acc, dp0 + off, dq0 + off, colP, colQ + shiftQ, 4, steps, i == 0);
+                mmaCommit(empty + 8 * s);
+                if (i + 1 == n) mmaCommit(done);
             }
-            const unsigned long long dp = operandDesc(at), dq = operandDesc(at + S::bytesP);
-            for (int i = 0; i < steps; ++i) {
-                // mxfp4: a word of four scales reaches over 128 elements, two steps; nvfp4: over one
-                const int c = NV ? i : i >> 1, pair = NV ? 0 : (i & 1) * 2;
-                mma<NV>(acc, dp + i * 2, dq + i * 2, instruction<BN, NV>(pair), colP + c * 4, colQ + c * 4 * S::rowTilesQ,
-                        kt > 0 || i > 0);
-            }
-            mmaCommit(empty + 8 * s);
+            __syncwarp();
+            if (++s == S::stages) s = 0, phase ^= 1;
         }
-        mmaCommit(done);
-    } else if (warp < 4) {
-        const bool finished = barWait(done, 0, stalled) && !*stalled;
-        if (__all_sync(0xFFFFFFFFu, finished)) {  // the reads below are the whole warp's
+    }
+    const bool finished = warp < 4 && __all_sync(0xFFFFFFFFu, barWait(done, 0, stalled) && !*stalled);  // the reads are the whole warp's
+    const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
+    const unsigned int mine = acc + (static_cast<unsigned int>(warp * 32) << 16);
+    const int row = warp * 32 + lane;
+    if (g.split == 1) {
+        if (finished) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
-            const unsigned int mine = acc + (static_cast<unsigned int>(warp * 32) << 16);
-            const long long p = p0 + warp * 32 + lane;
             if (g.outTag == T_F16) {
-                epilogue<__half, BN>(g, mine, p, q0, alpha);
+                epilogue<__half, BN>(g, mine, p0 + row, q0, alpha);
             } else if (g.outTag == T_BF16) {
-                epilogue<__nv_bfloat16, BN>(g, mine, p, q0, alpha);
+                epilogue<__nv_bfloat16, BN>(g, mine, p0 + row, q0, alpha);
             } else {
-                epilogue<float, BN>(g, mine, p, q0, alpha);
+                epilogue<float, BN>(g, mine, p0 + row, q0, alpha);
             }
         }
+    } else {
+        if (finished) {  // all products are done with the stages
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            constexpr int w = BN < 32 ? BN : 32;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += w) {
+                float v[32];
+                if (w == 32) {
+                    readColumns(mine + c, v);
+                } else {
+                    readColumns16(mine + c, v);
+                }
+#pragma unroll
+                for (int i = 0; i < w; ++i) {
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(stage0 + ((c + i) * 128 + row) * 4), "f"(v[i]) : "memory");
+                }
+            }
+        }
+        __syncwarp();
+        clusterSync();
+        if (finished) {
+            if (g.outTag == T_F16) {
+                joinColumns<__half, BN>(g, stage0, rank, row, p0 + row, q0, alpha);
+            } else if (g.outTag == T_BF16) {
+                joinColumns<__nv_bfloat16, BN>(g, stage0, rank, row, p0 + row, q0, alpha);
+            } else {
+                joinColumns<float, BN>(g, stage0, rank, row, p0 + row, q0, alpha);
+            }
+        }
+        __syncwarp();
+        clusterSync();  // the others have read this CTA's sums
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 5) {
-        __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmemBase), "r"(S::cols) : "memory");
+    }
+    if (threadIdx.x == 0 && *stalled) atomicCAS(g.err, E_NONE, E_STALLED);
+}
+
+// Tile t of the sweep: eight tiles of P down, then on to the next of Q, so that the tiles in flight form a
+// block and share their operands in L2.
+__device__ __forceinline__ void tileOf(const MxMatmulParams& g, int t, int* p, int* q) {
+    constexpr int G = 8;
+    const int group = t / (G * g.tilesQ), r = t - group * G * g.tilesQ;
+    const int high = min(G, g.tilesP - group * G);
+    *q = r / high;
+    *p = group * G + (r - *q * high);
+}
+
+template <class T>
+__device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, unsigned int acc, int buf, long long p, long long q0, float alpha,
+                                             unsigned int accFree, int lane) {
+    // columns 160..255 of tensor memory belong to both buffers: they are read first, and the next tile may start
+    const int shared0 = buf ? 0 : 160;
+    float v[3][32];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) readColumns(acc + shared0 + i * 32, v[i]);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(accFree) : "memory");
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[i][j] = v[i][j] * alpha;
+        storeColumns<T, 32>(g, p, q0 + shared0 + i * 32, v[i]);
+    }
+    const int rest = buf ? 96 : 0;
+#pragma unroll 1
+    for (int c = 0; c < 160; c += 32) {
+        readColumns(acc + rest + c, v[0]);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[0][j] = v[0][j] * alpha;
+        storeColumns<T, 32>(g, p, q0 + rest + c, v[0]);
+    }
+}
+
+template <bool NV>
+__global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
+                                                               const __grid_constant__ CUtensorMap mapScalesP,
+                                                               const __grid_constant__ CUtensorMap mapScalesQ,
+                                                               const __grid_constant__ MxMatmulParams g) {
+    typedef PairTile<NV> S;
+    extern __shared__ unsigned char raw[];
+    __shared__ unsigned long long bars[2 * S::stages + 2];
+    __shared__ unsigned int tmemBase;
+    __shared__ int stalledWord;
+    volatile int* stalled = &stalledWord;
+    const unsigned int stage0 = (smemAddr(raw) + 1023u) & ~1023u;
+    const unsigned int full = smemAddr(bars), empty = full + 8 * S::stages, accFull = empty + 8 * S::stages, accFree = accFull + 8;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const unsigned int rank = clusterRank();
+    const int tiles = g.tilesP * g.tilesQ, pairs = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::stages; ++s) {
+            barInit(full + 8 * s, 1);
+            barInit(empty + 8 * s, 1);
+        }
+        barInit(accFull, 1);
+        barInit(accFree, 8);  // four epilogue warps of both CTAs
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        stalledWord = 0;
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&tmemBase)), "r"(S::cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    clusterSync();  // both CTAs' barriers are there
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned int tmem = tmemBase;
+
+    if (warp == 4) {
+        // each CTA loads its halves; what they bring is counted at the first CTA's barrier, where the products wait
+        const unsigned int full0 = addrIn(full, 0);
+        int s = 0, phase = 1, issued = 0;
+        bool ok = true;
+        for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs) {
+            int tp, tq;
+            tileOf(g, t, &tp, &tq);
+            for (int kt = 0; kt < g.ktiles; ++kt, ++issued) {
+                ok = __all_sync(0xFFFFFFFFu, issued < S::stages || barWait(empty + 8 * s, phase, stalled));
+                if (!ok) break;
+                if (electOne()) {
+                    const unsigned int at = stage0 + s * S::stageBytes, bar = full0 + 8 * s;
+                    if (rank == 0) expectBytes(full + 8 * s, 2 * (2 * S::bytesSide + 3 * S::scaleBytes));
+                    loadTilePair(at, &mapP, kt * 128, tp * 256 + static_cast<int>(rank) * 128, bar);
+                    loadTilePair(at + S::bytesSide, &mapQ, kt * 128, tq * 256 + static_cast<int>(rank) * 128, bar);
+                    const unsigned int sp = at + 2 * S::bytesSide;
+                    loadScalesPair(sp, &mapScalesP, kt * S::chunksPerTile, tp * 2 + static_cast<int>(rank), bar);
+                    loadScalesPair(sp + S::scaleBytes, &mapScalesQ, kt * S::chunksPerTile, tq * 2, bar);
+                }
+                __syncwarp();
+                if (++s == S::stages) s = 0, phase ^= 1;
+            }
+        }
+        if (*stalled && rank == 0) {  // copies in flight write both CTAs' memory, which stays until they have
+            for (int i = max(0, issued - S::stages); i < issued; ++i) drain(full + 8 * (i % S::stages), (i / S::stages) & 1);
+        }
+    } else if (warp == 5 && rank == 0) {
+        const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesSide);
+        const unsigned long long ds0 = scaleDesc(stage0 + 2 * S::bytesSide);
+        int s = 0, phase = 0, it = 0, done = 0;
+        bool ok = true;
+        for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs, ++done) {
+            const unsigned int acc = tmem + (done & 1) * S::accStep;
+            if (done > 0) ok = __all_sync(0xFFFFFFFFu, barWait(accFree, (done - 1) & 1, stalled));
+            for (int kt = 0; kt < g.ktiles && ok; ++kt, ++it) {
+                ok = barWait(full + 8 * s, phase, stalled);
+                // as above: a copy of scales waits for the products that read the columns before
+                if (it >= S::scaleBufs) ok = ok && barWait(empty + 8 * ((it - S::scaleBufs) % S::stages), ((it - S::scaleBufs) / S::stages) & 1, stalled);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (electOne()) {
+                    const unsigned int colP = tmem + S::scaleCol + (it % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
+                    const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
+                    const int steps = kt + 1 < g.ktiles ? kTileK / kStepK
+                                                        : static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+#pragma unroll
+                    for (int c = 0; c < S::chunksPerTile; ++c) {
+                        copyScalesPair(colP + c * 4, ds0 + off + c * 32);
+                        copyScalesPair(colQ + c * 8, ds0 + off + S::scaleBytes / 16 + c * 32);
+                        copyScalesPair(colQ + c * 8 + 4, ds0 + off + S::scaleBytes / 8 + c * 32);
+                    }
+                    mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, steps, kt == 0);
+                    mmaCommitPair(empty + 8 * s);
+                    if (kt + 1 == g.ktiles) mmaCommitPair(accFull);
+                }
+                __syncwarp();
+                if (++s == S::stages) s = 0, phase ^= 1;
+            }
+        }
+    } else if (warp < 4) {
+        const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
+        const unsigned int accFree0 = addrIn(accFree, 0);
+        int done = 0;
+        for (int t = blockIdx.x / 2; t < tiles; t += pairs, ++done) {
+            int tp, tq;
+            tileOf(g, t, &tp, &tq);
+            if (!__all_sync(0xFFFFFFFFu, barWait(accFull, done & 1, stalled) && !*stalled)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int buf = done & 1;
+            const unsigned int acc = tmem + buf * S::accStep + (static_cast<unsigned int>(warp * 32) << 16);
+            const long long p = static_cast<long long>(tp) * 256 + rank * 128 + warp * 32 + lane, q0 = static_cast<long long>(tq) * 256;
+            if (g.outTag == T_F16) {
+                pairEpilogue<__half>(g, acc, buf, p, q0, alpha, accFree0, lane);
+            } else if (g.outTag == T_BF16) {
+                pairEpilogue<__nv_bfloat16>(g, acc, buf, p, q0, alpha, accFree0, lane);
+            } else {
+                pairEpilogue<float>(g, acc, buf, p, q0, alpha, accFree0, lane);
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    clusterSync();  // neither CTA leaves while the other's products, copies or arrivals reach into it
+    if (warp == 5) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmemBase), "r"(S::cols) : "memory");
     }
     if (threadIdx.x == 0 && *stalled) atomicCAS(g.err, E_NONE, E_STALLED);
 }
@@ -387,22 +694,76 @@ CUtensorMap mapOf(const b200c_mx_matrix& m, int boxRows) {
     return map;
 }
 
+// Scales as [row tiles][block tiles][512 bytes]; what lies behind either end is read as 0.
+CUtensorMap scaleMapOf(const b200c_mx_matrix& m, int chunksPerTile, int boxTiles) {
+    CUtensorMap map;
+    const cuuint64_t chunks = static_cast<cuuint64_t>((mxBlocks(m.format, m.cols) + 3) / 4);
+    const cuuint64_t dims[3] = {256, chunks, static_cast<cuuint64_t>((m.rows + 127) / 128)};
+    const cuuint64_t strides[2] = {512, chunks * 512};
+    const cuuint32_t box[3] = {256, static_cast<cuuint32_t>(chunksPerTile), static_cast<cuuint32_t>(boxTiles)};
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUresult r = encodeTiled()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, m.scales, dims, strides, box, step,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw CudaFail("cuTensorMapEncodeTiled failed with " + std::to_string(static_cast<int>(r)));
+    return map;
+}
+
+// The kernel may use `bytes` of shared memory; told once per device.
+template <class Kernel>
+void allowSmem(Context* ctx, Kernel kernel, int bytes, std::atomic<unsigned long long>& ready) {
+    const unsigned long long bit = 1ull << (ctx->device & 63);
+    if (ready.load() & bit) return;
+    B2_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready.fetch_or(bit);
+}
+
+template <class... Args>
+void launchClusters(Context* ctx, void (*kernel)(Args...), unsigned int ctas, unsigned int perCluster, int smem,
+                    typename std::common_type<Args>::type... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = perCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    ++ctx->launches;
+}
+
 template <int BN, bool NV>
 void launchTileOf(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix& q, MxMatmulParams g) {
     typedef Tile<BN, NV> S;
-    static std::atomic<unsigned long long> ready{0};  // devices that have been told of the shared memory
-    const unsigned long long bit = 1ull << (ctx->device & 63);
-    if (!(ready.load() & bit)) {
-        B2_CUDA(cudaFuncSetAttribute(mxMatmulKernel<BN, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smemBytes));
-        ready.fetch_or(bit);
-    }
-    const CUtensorMap mapP = mapOf(p, 128), mapQ = mapOf(q, BN);
+    static std::atomic<unsigned long long> ready{0};
+    allowSmem(ctx, mxMatmulKernel<BN, NV>, S::smemBytes, ready);
+    g.tilesP = static_cast<int>((p.rows + 127) / 128);
     g.tilesQ = static_cast<int>((q.rows + BN - 1) / BN);
-    const long long tiles = (p.rows + 127) / 128 * g.tilesQ;
-    if (tiles > 0x7FFFFFFFll) throw BadArg("the product has too many tiles");
-    mxMatmulKernel<BN, NV><<<static_cast<unsigned int>(tiles), kThreads, S::smemBytes, ctx->stream>>>(mapP, mapQ, g);
-    B2_CUDA(cudaGetLastError());
-    ++ctx->launches;
+    const long long tiles = static_cast<long long>(g.tilesP) * g.tilesQ;
+    // two CTAs per SM: k is shared out while there are CTAs to spare and each keeps two stages' worth
+    g.split = 1;
+    while (g.split < 8 && tiles * g.split * 2 <= 2 * ctx->smCount && g.ktiles >= 4 * g.split) g.split *= 2;
+    if (tiles * g.split > 0x7FFFFFFFll) throw BadArg("the product has too many tiles");
+    launchClusters(ctx, mxMatmulKernel<BN, NV>, static_cast<unsigned int>(tiles * g.split), static_cast<unsigned int>(g.split), S::smemBytes,
+                   mapOf(p, 128), mapOf(q, BN), g);
+}
+
+template <bool NV>
+void launchPairs(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix& q, MxMatmulParams g) {
+    typedef PairTile<NV> S;
+    static std::atomic<unsigned long long> ready{0};
+    allowSmem(ctx, mxMatmulPairKernel<NV>, S::smemBytes, ready);
+    g.tilesP = static_cast<int>((p.rows + 255) / 256);
+    g.tilesQ = static_cast<int>((q.rows + 255) / 256);
+    const long long tiles = static_cast<long long>(g.tilesP) * g.tilesQ;
+    if (tiles > 0x3FFFFFFFll) throw BadArg("the product has too many tiles");
+    const long long pairs = std::min<long long>(tiles, ctx->smCount / 2);
+    launchClusters(ctx, mxMatmulPairKernel<NV>, static_cast<unsigned int>(2 * pairs), 2u, S::smemBytes, mapOf(p, 128), mapOf(q, 128),
+                   scaleMapOf(p, S::chunksPerTile, 1), scaleMapOf(q, S::chunksPerTile, 2), g);
 }
 
 template <int BN>
@@ -425,8 +786,9 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
                                   ctx->stream));
         return;
     }
-    // a side of up to 128 rows becomes the columns of a tile, which may be few
-    const bool across = a.rows <= 128 && a.rows < b.rows;
+    const long long big = ((a.rows + 255) / 256) * ((b.rows + 255) / 256);
+    const bool pairs = big >= ctx->smCount / 4 && a.rows > 128 && b.rows > 128;
+    const bool across = !pairs && a.rows < b.rows;
     const b200c_mx_matrix& p = across ? b : a;
     const b200c_mx_matrix& q = across ? a : b;
     const bool nv = a.format == B200C_NVFP4;
@@ -441,21 +803,28 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     g.chunks = (mxBlocks(a.format, a.cols) + 3) / 4;
     g.scaleTilesQ = static_cast<int>((q.rows + 127) / 128);
     g.ktiles = static_cast<int>((a.cols + kTileK - 1) / kTileK);
-    g.tilesQ = 0;
+    g.tilesP = g.tilesQ = 0;
+    g.split = 1;
     g.out = out;
     g.ld = outLd;
     g.outTag = dtype == B200C_F16 ? T_F16 : dtype == B200C_BF16 ? T_BF16 : T_F32;
     g.across = across;
     g.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (outLd * es) % 16 == 0;
     g.err = ctx->errWord;
-    if (q.rows <= 16) {
+    if (pairs) {
+        if (nv) {
+            launchPairs<true>(ctx, p, q, g);
+        } else {
+            launchPairs<false>(ctx, p, q, g);
+        }
+    } else if (q.rows <= 16) {
         launchFormat<16>(ctx, p, q, g);
+    } else if (q.rows <= 32) {
+        launchFormat<32>(ctx, p, q, g);
     } else if (q.rows <= 64) {
         launchFormat<64>(ctx, p, q, g);
-    } else if (q.rows <= 128) {
-        launchFormat<128>(ctx, p, q, g);
     } else {
-        launchFormat<256>(ctx, p, q, g);
+        launchFormat<128>(ctx, p, q, g);
     }
 }
 

@@ -305,7 +305,9 @@ def check_product(got, va, vb, dtype):
 
 
 PRODUCTS = [(1, 1, 1), (1, 128, 32), (3, 5, 16), (16, 130, 100), (17, 300, 257), (64, 64, 64), (65, 1000, 515), (128, 129, 300),
-            (129, 128, 1003), (200, 300, 4100), (300, 20, 777), (257, 513, 2048), (1, 1000, 11008), (130, 1, 96)]
+            (129, 128, 1003), (200, 300, 4100), (300, 20, 777), (257, 513, 2048), (1, 1000, 11008), (130, 1, 96),
+            # from here on the two-CTA form: a stage and less, several tiles per pair, ragged edges
+            (1537, 1700, 40), (1537, 1700, 1003), (257, 4900, 515), (2600, 2700, 300), (4864, 257, 2048)]
 
 
 @pytest.mark.gpu
@@ -324,7 +326,7 @@ def test_matmul(dev, fmt, m, n, k):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(16, 256, 1024), (300, 700, 2048)])
+@pytest.mark.parametrize("m,n,k", [(16, 256, 1024), (300, 700, 2048), (1600, 1800, 2048)])
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_matmul_is_exact_where_sums_are(dev, fmt, m, n, k):
     """Scales of one: every product is a multiple of 1/4 below 36, so sums of up to 2^17 of them fit 24 bits."""
@@ -342,10 +344,10 @@ def test_matmul_is_exact_where_sums_are(dev, fmt, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(20, 150, 200), (1700, 1601, 200)])
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_matmul_keeps_nan_to_its_rows(dev, fmt):
+def test_matmul_keeps_nan_to_its_rows(dev, fmt, m, n, k):
     """A NaN scale in one row of each side; the scales that fill up the tiles are NaN too, and must not matter."""
-    m, n, k = 20, 150, 200
     a, va = random_held(fmt, m, k, 1)
     b, vb = random_held(fmt, n, k, 2)
     nan = 255 if fmt == A.MXFP4 else 127
