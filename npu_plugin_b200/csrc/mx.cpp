@@ -8,7 +8,7 @@ namespace b200c {
 namespace {
 
 // A row or column index fits 31 bits with room to round up to a tile; offsets are 64 bits everywhere.
-constexpr int64_t kMaxExtent = 0x7FFFFFFF - 1024;
+constexpr int64_t kMaxExtent = 0x7FFFFFFF - 65536;
 
 struct Range {
     const char* what;

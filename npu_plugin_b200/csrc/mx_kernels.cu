@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200c {
 
@@ -29,7 +30,6 @@ struct MxQuantParams {
     long long blocks;       // blocks of a row
     long long scaleRows;    // rows of scale bytes, those that fill up the last tile included
     long long scaleBlocks;  // the same for blocks
-    int wideIn, wideValues;  // 16-byte accesses are aligned
 };
 
 struct MxDequantParams {
@@ -41,7 +41,6 @@ struct MxDequantParams {
     long long rows, cols, blocks;
     void* out;
     long long outLd;
-    int wideOut;
 };
 
 __device__ __forceinline__ long long scaleAt(int tiled, long long row, long long block, long long blocks) {
@@ -79,17 +78,32 @@ __device__ __forceinline__ float fromFloat<float>(float v) {
     return v;
 }
 
-// two 32-bit values -> two codes in a byte, `lo` in the low nibble: nearest even, at most 6
-__device__ __forceinline__ unsigned int codePair(float lo, float hi) {
+// eight 32-bit values -> eight codes, the first in the lowest nibble: nearest even, at most 6
+__device__ __forceinline__ unsigned int codesOf(const float v[8]) {
     unsigned int r;
-    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
-// a byte of two codes -> their values in f16 (exact)
-__device__ __forceinline__ float2 codeValues(unsigned int byte) {
-    unsigned int h;
-    asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(h) : "r"(byte));
-    return __half22float2(*reinterpret_cast<__half2*>(&h));
+// eight codes -> their values in f16 (exact), two to a word
+__device__ __forceinline__ void valuesOf(unsigned int word, __half2 h[4]) {
+    unsigned int r[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+        : "r"(word));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2*>(&r[i]);
 }
 __device__ __forceinline__ unsigned int toE4m3(float v) {
     unsigned short r;
@@ -106,34 +120,76 @@ __device__ __forceinline__ float fromE8m0(unsigned int byte) {
     return byte == 255u ? __uint_as_float(0x7FFFFFFFu) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
 }
 
+// 8 elements as they lie in memory
 template <class T>
-__device__ __forceinline__ void load8(const T* p, bool wide, long long left, float v[8]) {
-    if (wide && left >= 8) {
-        alignas(16) T t[8];
-        constexpr int n = 8 * sizeof(T) / 16;
+struct Raw {
+    static constexpr int n = 8 * sizeof(T) / 16;
+    uint4 v[n];
+};
+// `wide`: 16-byte loads are aligned.  Behind the last column: zeros.
+template <class T, bool WIDE>
+__device__ __forceinline__ Raw<T> load8(const T* p, int left) {
+    Raw<T> r;
+    if (WIDE) {  // all eight or none
 #pragma unroll
-        for (int i = 0; i < n; ++i) reinterpret_cast<uint4*>(t)[i] = reinterpret_cast<const uint4*>(p)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = toFloat<T>(t[i]);
+        for (int i = 0; i < Raw<T>::n; ++i) r.v[i] = left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
     } else {
+        T* t = reinterpret_cast<T*>(r.v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? toFloat<T>(p[i]) : 0.f;
+        for (int i = 0; i < 8; ++i) t[i] = i < left ? p[i] : fromFloat<T>(0.f);
     }
+    return r;
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, bool wide, long long left, const float v[8]) {
-    if (wide && left >= 8) {
-        alignas(16) T t[8];
-        constexpr int n = 8 * sizeof(T) / 16;
+__device__ __forceinline__ void unpack8(const Raw<T>& r, float v[8]) {
+    const T* t = reinterpret_cast<const T*>(r.v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = fromFloat<T>(v[i]);
+    for (int i = 0; i < 8; ++i) v[i] = toFloat<T>(t[i]);
+}
+// what eight codes with the factor d stand for -> p.  `power`: d is a power of two
+template <class T, bool WIDE, bool POWER>
+__device__ __forceinline__ void storeValues(T* p, int left, unsigned int word, float d) {
+    __half2 h[4];
+    valuesOf(word, h);
+    alignas(16) T t[8];
+    if (sizeof(T) == 2 && POWER && std::is_same<T, __half>::value && d >= 5.9604645e-8f && d <= 32768.f) {
+        // a factor that f16 has: the product is rounded once, and only where it is subnormal or too large
+        const __half2 f = __half2half2(__float2half_rn(d));
 #pragma unroll
-        for (int i = 0; i < n; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(t)[i];
+        for (int i = 0; i < 4; ++i) reinterpret_cast<__half2*>(t)[i] = __hmul2(h[i], f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 c = __half22float2(h[i]);
+            t[2 * i] = fromFloat<T>(c.x * d);
+            t[2 * i + 1] = fromFloat<T>(c.y * d);
+        }
+    }
+    if (WIDE) {
+#pragma unroll
+        for (int i = 0; i < Raw<T>::n; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(t)[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = fromFloat<T>(v[i]);
+            if (i < left) p[i] = t[i];
     }
+}
+// largest magnitude of the eight, as the bits of a 32-bit float: bits of magnitudes order like the magnitudes,
+// for 16-bit types two at a time
+template <class T>
+__device__ __forceinline__ unsigned int top8(const Raw<T>& r) {
+    const unsigned int* w = reinterpret_cast<const unsigned int*>(r.v);
+    if (sizeof(T) == 2) {
+        unsigned int m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        const unsigned short h = static_cast<unsigned short>(max(m >> 16, m & 0xFFFFu));
+        return __float_as_uint(toFloat<T>(*reinterpret_cast<const T*>(&h)));
+    }
+    unsigned int m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+    return m;
 }
 
 // the smallest power of two t >= 2^-126 with top <= 2688 t; 2688 = 1.3125 * 2^11, so t = 2^(e - 11) when top's
@@ -145,21 +201,53 @@ __device__ __forceinline__ float tensorScaleOf(float top) {
     return __uint_as_float(static_cast<unsigned int>(max(e, 1)) << 23);
 }
 
-// largest finite magnitude of the matrix -> tensorScale[1] (zeroed before).  Magnitudes compare like
-// their bits, and a maximum does not depend on the order it is taken in.
-template <class T>
+constexpr int kUnits = 4;  // units of a thread where rows are long
+
+// How a kernel's threads lie over rows x units (8 elements): x along a row, y over rows, each thread with UNITS
+// units of one row, x apart, whose loads are all under way before the first is used.  Addresses differ by
+// constants between a thread's units: with its units in different rows instead, 64-bit address arithmetic was a
+// quarter of all instructions.
+template <int UNITS>
+struct Lay {
+    static constexpr int wide = 128;  // x of a thread with several units
+    __device__ __forceinline__ static int x() {
+        return UNITS > 1 ? wide : static_cast<int>(blockDim.x);
+    }
+    __device__ __forceinline__ static int firstUnit() {
+        return static_cast<int>(blockIdx.y) * x() * UNITS + static_cast<int>(threadIdx.x);
+    }
+    __device__ __forceinline__ static int unitStep() {  // on to the next part of a row longer than the grid
+        return static_cast<int>(gridDim.y) * x() * UNITS;
+    }
+};
+
+// largest finite magnitude of the matrix -> tensorScale[1] (zeroed before).  A maximum does not depend on the
+// order it is taken in.
+template <class T, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQuantParams p) {
+    typedef Lay<UNITS> L;
     unsigned int top = 0;
-    const long long units = (p.cols + 7) / 8;
-    for (long long r = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; r < p.rows; r += static_cast<long long>(gridDim.y) * blockDim.y) {
-        const T* row = static_cast<const T*>(p.src) + r * p.srcLd;
-        for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < units; u += static_cast<long long>(gridDim.x) * blockDim.x) {
-            float v[8];
-            load8<T>(row + u * 8, p.wideIn != 0, p.cols - u * 8, v);
+    const int units = static_cast<int>((p.cols + 7) / 8), cols = static_cast<int>(p.cols);
+    for (long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; r < p.rows; r += static_cast<long long>(gridDim.x) * blockDim.y) {
+        for (int u = L::firstUnit(); u < units; u += L::unitStep()) {
+            const T* src = static_cast<const T*>(p.src) + r * p.srcLd + u * 8ll;
+            Raw<T> raw[UNITS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned int a = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-                if (a < 0x7F800000u) top = max(top, a);
+            for (int i = 0; i < UNITS; ++i) raw[i] = load8<T, WIDE>(src + i * L::x() * 8, cols - 8 * (u + i * L::x()));
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const unsigned int m = top8<T>(raw[i]);
+                if (m < 0x7F800000u) {
+                    top = max(top, m);
+                } else {  // a NaN or an infinity hides the others
+                    float v[8];
+                    unpack8<T>(raw[i], v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const unsigned int a = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+                        if (a < 0x7F800000u) top = max(top, a);
+                    }
+                }
             }
         }
     }
@@ -167,8 +255,84 @@ __global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQua
     if (((threadIdx.y * blockDim.x + threadIdx.x) & 31) == 0 && top) atomicMax(reinterpret_cast<unsigned int*>(p.tensorScale) + 1, top);
 }
 
+// v / d in 32 bits without the divide instruction's calls: the product with 1 / d, corrected once by its
+// remainder, is the rounded quotient where the remainder is exact -- for d and v within 2^-60 .. 2^60; quotients
+// below 2^-20, for which it may not be, are the code and the scale 0 either way.  Otherwise d is brought to
+// 1 .. 2 first and v along with it; what then leaves 32 bits is far above the largest code or below the smallest.
+struct Divisor {
+    float d, r, s1, s2;
+    bool far;
+    __device__ __forceinline__ Divisor(float by, float top): d(by), s1(1.f), s2(1.f) {
+        far = !(by >= 8.6736174e-19f && by <= 1.1529215e18f && top <= 1.1529215e18f);
+        if (far) {
+            if (by <= 3.402823466e38f) {
+                const float n = by < 1.1754944e-38f ? by * 16777216.f : by;  // subnormal numbers have no exponent field
+                const int e = static_cast<int>(__float_as_uint(n) >> 23) - 127 - (by < 1.1754944e-38f ? 24 : 0);
+                const int h = -e / 2;
+                s1 = __uint_as_float(static_cast<unsigned int>(h + 127) << 23);
+                s2 = __uint_as_float(static_cast<unsigned int>(-e - h + 127) << 23);
+                d = by * s1 * s2;
+            } else {  // infinity: all quotients are 0
+                s1 = 0.f;
+                d = 1.f;
+            }
+        }
+        float r0;  // one Newton step from an approximation: 1 / d to the last bit or nearly so
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(d));
+        r = __fmaf_rn(__fmaf_rn(-d, r0, 1.f), r0, r0);
+    }
+    __device__ __forceinline__ float near(float v) const {
+        const float q = __fmul_rn(v, r);
+        return copysignf(__fmaf_rn(__fmaf_rn(-q, d, v), r, q), v);  // a zero would lose its sign
+    }
+    __device__ __forceinline__ float within(float v) const {
+        return fminf(fmaxf(v * s1 * s2, -1e30f), 1e30f);
+    }
+};
+
+// Eight elements of a block whose largest magnitude is `top` -> their codes; the block's scale and the factor of
+// its codes (which makes NaN of the codes of a block with a NaN or an infinity).
 template <class T, bool NV>
-__global__ void __launch_bounds__(256) mxQuantKernel(const __grid_constant__ MxQuantParams p) {
+__device__ __forceinline__ unsigned int encode8(const Raw<T>& raw, unsigned int top, float t, const Divisor& sixT, bool badT, unsigned int* scaleByte,
+                                                float* factor) {
+    const bool poison = top >= 0x7F800000u;
+    float v[8];
+    unpack8<T>(raw, v);
+    bool zero = poison;
+    if (!NV) {
+        // the exponent field of the largest magnitude, less 2; subnormal numbers have the field 0
+        const unsigned int scale = poison ? 0xFFu : static_cast<unsigned int>(max(static_cast<int>(top >> 23) - 2, 0));
+        const float up = __uint_as_float((254u << 23) - (scale << 23));  // 2^-X
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * up;
+        *scaleByte = scale;
+        // 2^X, a subnormal number for the byte 0; infinity for 0xFF, and the codes are 0
+        *factor = __uint_as_float(max(scale << 23, 0x00400000u));
+    } else {
+        const float m = __uint_as_float(top);
+        const float s = sixT.near(sixT.far || !(m <= 1.1529215e18f) ? sixT.within(m) : m);
+        const unsigned int scale = poison || badT ? 0x7Fu : toE4m3(fminf(s, 448.f));
+        const float d = __fmul_rn(fromE4m3(scale), t);
+        zero = scale == 0x7Fu || !(d > 0.f);
+        const Divisor by(d, m);
+        if (by.far) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = by.within(v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = by.near(v[i]);
+        *scaleByte = scale;
+        *factor = d;
+    }
+    const unsigned int word = codesOf(v);
+    return zero ? 0u : word;
+}
+
+// Whole warps go through the loop together, whatever their rows.  The last CTAs of the grid (blockIdx.x >=
+// rowCtas) zero the scales of the rows that only fill a tile up.
+template <class T, bool NV, bool WIDE, bool VALUES, int UNITS>
+__global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ MxQuantParams p, int rowCtas) {
+    typedef Lay<UNITS> L;
     float t = 1.f;
     if (NV) {
         if (p.scaleGiven) {
@@ -178,123 +342,181 @@ __global__ void __launch_bounds__(256) mxQuantKernel(const __grid_constant__ MxQ
             if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && threadIdx.y == 0) p.tensorScale[0] = t;
         }
     }
+    const Divisor sixT(NV ? 6.f * t : 1.f, 0.f);
+    const bool badT = NV && !(t > 0.f && t <= 3.402823466e38f);
     constexpr int lanes = NV ? 2 : 4;  // threads of a block
-    const long long units = (p.cols + 31) / 32 * 4;               // words of codes in a row
-    const long long all = max(units, p.scaleBlocks * lanes);      // and those that only write a tile's filling scales
-    for (long long r = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; r < p.scaleRows; r += static_cast<long long>(gridDim.y) * blockDim.y) {
-        const T* row = static_cast<const T*>(p.src) + r * p.srcLd;
-        // a group of four threads runs the loop together: `all` and blockDim.x are multiples of 4
-        for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < all; u += static_cast<long long>(gridDim.x) * blockDim.x) {
-            float v[8];
-            const long long left = r < p.rows ? p.cols - u * 8 : 0;
-            load8<T>(row + u * 8, p.wideIn != 0, left, v);
-            unsigned int top = 0;
+    if (static_cast<int>(blockIdx.x) >= rowCtas) {
+        const int threads = blockDim.x * blockDim.y;
+        const long long chunks = p.scaleBlocks / 4, n = (p.scaleRows - p.rows) * chunks;
+        const long long cta = static_cast<long long>(blockIdx.x - rowCtas) * gridDim.y + blockIdx.y;
+        const long long all = static_cast<long long>(gridDim.x - rowCtas) * gridDim.y * threads;
+        for (long long i = cta * threads + threadIdx.y * blockDim.x + threadIdx.x; i < n; i += all) {
+            *reinterpret_cast<unsigned int*>(p.scales + scaleAt(1, p.rows + i / chunks, i % chunks * 4, p.blocks)) = 0u;
+        }
+        return;
+    }
+    const int cols = static_cast<int>(p.cols), units = (cols + 31) / 32 * 4;
+    const int all = max(units, static_cast<int>(p.scaleBlocks) * lanes);  // those of a tile's filling scales too
+    // from the last row to the first: where the largest magnitude was looked for just before, the last rows are
+    // what L2 still holds
+    const long long r = p.rows - 1 - (static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y);
+    const T* src = static_cast<const T*>(p.src) + r * p.srcLd;
+    unsigned char* codes = p.codes + r * p.ld;
+    T* values = static_cast<T*>(p.values) + r * p.valuesLd;
+    // tiled: blocks of four lie 512 bytes apart
+    unsigned char* scales = p.scales + (r >= 0 ? scaleAt(p.tiled, r, 0, p.blocks) : 0);
+    const int begin = L::firstUnit() - static_cast<int>(threadIdx.x);
+    for (int base = begin; base < all; base += L::unitStep()) {
+        const int u = base + threadIdx.x;
+        Raw<T> raw[UNITS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-            const unsigned int group = 0xFu << (((threadIdx.y * blockDim.x + threadIdx.x) & 31) & ~3);
-            top = max(top, __shfl_xor_sync(group, top, 1));
-            if (!NV) top = max(top, __shfl_xor_sync(group, top, 2));
-
-            const bool poison = top >= 0x7F800000u;  // a NaN or an infinity in the block
+        for (int i = 0; i < UNITS; ++i) raw[i] = load8<T, WIDE>(src + u * 8ll + i * L::x() * 8, r >= 0 ? cols - 8 * (u + i * L::x()) : 0);
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int ui = u + i * L::x(), left = cols - 8 * ui;
+            unsigned int top = top8<T>(raw[i]);
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            if (!NV) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            float d;
             unsigned int scale;
-            float d, q[8];
-            bool zero = poison;
-            if (!NV) {
-                // the exponent field of the largest magnitude, less 2; subnormal numbers have the field 0
-                scale = poison ? 0xFFu : static_cast<unsigned int>(max(static_cast<int>(top >> 23) - 2, 0));
-                d = fromE8m0(scale);
-                const float up = __uint_as_float((254u - min(scale, 253u)) << 23);  // 2^-X
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] = v[i] * up;
-            } else {
-                // 0 / 0 and a NaN t fall to the scale NaN
-                const float s = __fdiv_rn(__uint_as_float(top), 6.f * t);
-                scale = poison || !(t > 0.f) || !(t <= 3.402823466e38f) ? 0x7Fu : toE4m3(fminf(s, 448.f));
-                d = __fmul_rn(fromE4m3(scale), t);
-                zero = scale == 0x7Fu || !(d > 0.f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[i], d);
-            }
-            unsigned int word = 0;
-            if (!zero) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) word |= codePair(q[2 * i], q[2 * i + 1]) << (8 * i);
-            }
-            if (r < p.rows && u < units) *reinterpret_cast<unsigned int*>(p.codes + r * p.ld + u * 4) = word;
-            if ((u & (lanes - 1)) == 0) {
-                const long long b = u / lanes;
-                if (b < p.scaleBlocks) p.scales[scaleAt(p.tiled, r, b, p.blocks)] = static_cast<unsigned char>(left > 0 ? scale : 0u);
-            }
-            if (p.values && left > 0) {
-                float w[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 c = codeValues((word >> (8 * i)) & 0xFFu);
-                    w[2 * i] = c.x * d;
-                    w[2 * i + 1] = c.y * d;
+            const unsigned int word = encode8<T, NV>(raw[i], top, t, sixT, badT, &scale, &d);
+            if (r >= 0) {
+                const int b = ui / lanes;
+                if ((ui & (lanes - 1)) == 0 && b < p.scaleBlocks) {
+                    scales[p.tiled ? (b >> 2) * 512ll + (b & 3) : b] = static_cast<unsigned char>(left > 0 ? scale : 0u);
                 }
-                store8<T>(static_cast<T*>(p.values) + r * p.valuesLd + u * 8, p.wideValues != 0, left, w);
+                if (ui < units) *reinterpret_cast<unsigned int*>(codes + ui * 4ll) = word;
+                if (VALUES && left > 0) storeValues<T, WIDE, !NV>(values + ui * 8ll, left, word, d);
             }
         }
     }
 }
 
-template <class T, bool NV>
+template <class T, bool NV, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(256) mxDequantKernel(const __grid_constant__ MxDequantParams p) {
+    typedef Lay<UNITS> L;
     const float t = NV ? p.tensorScale[0] : 1.f;
-    const long long units = (p.cols + 7) / 8;
-    for (long long r = static_cast<long long>(blockIdx.y) * blockDim.y + threadIdx.y; r < p.rows; r += static_cast<long long>(gridDim.y) * blockDim.y) {
-        for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < units; u += static_cast<long long>(gridDim.x) * blockDim.x) {
-            const unsigned int word = *reinterpret_cast<const unsigned int*>(p.codes + r * p.ld + u * 4);
-            const unsigned int scale = p.scales[scaleAt(p.tiled, r, u / (NV ? 2 : 4), p.blocks)];
-            const float d = NV ? __fmul_rn(fromE4m3(scale), t) : fromE8m0(scale);
-            float w[8];
+    const int cols = static_cast<int>(p.cols), units = (cols + 7) / 8;
+    const long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (r >= p.rows) return;
+    const unsigned char* codes = p.codes + r * p.ld;
+    const unsigned char* scales = p.scales + scaleAt(p.tiled, r, 0, p.blocks);
+    T* out = static_cast<T*>(p.out) + r * p.outLd;
+    for (int u = L::firstUnit(); u < units; u += L::unitStep()) {
+        unsigned int word[UNITS], scale[UNITS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 c = codeValues((word >> (8 * i)) & 0xFFu);
-                w[2 * i] = c.x * d;
-                w[2 * i + 1] = c.y * d;
+        for (int i = 0; i < UNITS; ++i) {
+            const int ui = u + i * L::x();
+            if (ui < units) {
+                const int b = ui / (NV ? 2 : 4);
+                word[i] = __ldcs(reinterpret_cast<const unsigned int*>(codes + ui * 4ll));
+                scale[i] = scales[p.tiled ? (b >> 2) * 512ll + (b & 3) : b];
             }
-            store8<T>(static_cast<T*>(p.out) + r * p.outLd + u * 8, p.wideOut != 0, p.cols - u * 8, w);
+        }
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            const int ui = u + i * L::x();
+            if (ui < units) {
+                const float d = NV ? __fmul_rn(fromE4m3(scale[i]), t) : fromE8m0(scale[i]);
+                storeValues<T, WIDE, !NV>(out + ui * 8ll, cols - 8 * ui, word[i], d);
+            }
         }
     }
 }
 
-// rows x units of 8 elements over CTAs of 256 threads; threads of a CTA cover as much of a row as there is
-void gridFor(Context* ctx, long long rows, long long units, dim3* grid, dim3* block) {
+// rows x units of 8 elements over CTAs of up to 256 threads
+void gridFor(long long rows, long long units, int unitsOfThread, dim3* grid, dim3* block) {
     unsigned int x = 4;
-    while (x < 256 && x < units) x *= 2;
-    *block = dim3(x, 256 / x);
-    const long long gx = std::max<long long>(1, std::min<long long>((units + x - 1) / x, 1024));
-    const long long want = (rows + block->y - 1) / block->y;
-    const long long most = std::max<long long>(1, ctx->smCount * 64LL / gx);
-    *grid = dim3(static_cast<unsigned int>(gx), static_cast<unsigned int>(std::max<long long>(1, std::min<long long>(want, std::min<long long>(most, 65535)))));
+    if (unitsOfThread > 1) {
+        x = Lay<kUnits>::wide;
+    } else {
+        while (x < 256 && x < units) x *= 2;
+    }
+    *block = dim3(x, unitsOfThread > 1 ? 1 : 256 / x);
+    const long long along = static_cast<long long>(x) * unitsOfThread;
+    *grid = dim3(static_cast<unsigned int>(std::max<long long>(1, (rows + block->y - 1) / block->y)),
+                 static_cast<unsigned int>(std::max<long long>(1, std::min<long long>((units + along - 1) / along, 65535))));
 }
 
 bool aligned16(const void* p, long long ldBytes) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ldBytes % 16 == 0;
 }
 
-template <class T>
-void quantizeAs(Context* ctx, const MxQuantParams& p, bool nv) {
+// Several units a thread: where they leave few of its last ones idle, and enough threads to fill the SMs
+bool longRows(Context* ctx, long long rows, long long units) {
+    constexpr long long along = Lay<kUnits>::wide * kUnits;
+    const long long padded = (units + along - 1) / along * along;
+    return padded * 7 <= units * 8 && rows * units >= 256ll * kUnits * 4 * ctx->smCount;
+}
+
+template <class T, bool NV, bool WIDE, int UNITS>
+void launchQuant(Context* ctx, const MxQuantParams& p, long long units) {
     dim3 grid, block;
+    gridFor(p.rows, units, UNITS, &grid, &block);
+    const int rowCtas = static_cast<int>(grid.x);
+    if (p.scaleRows > p.rows) {
+        const long long words = (p.scaleRows - p.rows) * (p.scaleBlocks / 4), perX = static_cast<long long>(block.x) * block.y * grid.y;
+        grid.x += static_cast<unsigned int>(std::min<long long>((words + perX - 1) / perX, 1024));
+    }
+    if (p.values) {
+        mxQuantKernel<T, NV, WIDE, true, UNITS><<<grid, block, 0, ctx->stream>>>(p, rowCtas);
+    } else {
+        mxQuantKernel<T, NV, WIDE, false, UNITS><<<grid, block, 0, ctx->stream>>>(p, rowCtas);
+    }
+    B2_CUDA(cudaGetLastError());
+    ++ctx->launches;
+}
+
+template <class T, bool WIDE, int UNITS>
+void launchTop(Context* ctx, const MxQuantParams& p) {
+    dim3 grid, block;
+    gridFor(p.rows, (p.cols + 7) / 8, UNITS, &grid, &block);
+    grid.x = std::min<unsigned int>(grid.x, ctx->smCount * 16u);  // few warps end with an atomic
+    mxTopKernel<T, WIDE, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+    B2_CUDA(cudaGetLastError());
+    ++ctx->launches;
+}
+
+template <class T, bool WIDE, int UNITS>
+void quantizeWith(Context* ctx, const MxQuantParams& p, bool nv) {
     if (nv && !p.scaleGiven) {
         fillBytes(ctx, p.tensorScale, 0, 8);
-        if (p.rows > 0 && p.cols > 0) {
-            gridFor(ctx, p.rows, (p.cols + 7) / 8, &grid, &block);
-            mxTopKernel<T><<<grid, block, 0, ctx->stream>>>(p);
-            B2_CUDA(cudaGetLastError());
-            ++ctx->launches;
-        }
+        if (p.rows > 0 && p.cols > 0) launchTop<T, WIDE, UNITS>(ctx, p);
     }
     // an empty matrix has no scales, but its factor is still written
     const long long units = std::max((p.cols + 31) / 32 * 4, p.scaleBlocks * (nv ? 2 : 4));
-    if ((p.scaleRows == 0 || units == 0) && !(nv && !p.scaleGiven)) return;
-    gridFor(ctx, p.scaleRows, units, &grid, &block);
+    if ((p.rows == 0 || units == 0) && !(nv && !p.scaleGiven)) return;
     if (nv) {
-        mxQuantKernel<T, true><<<grid, block, 0, ctx->stream>>>(p);
+        launchQuant<T, true, WIDE, UNITS>(ctx, p, units);
     } else {
-        mxQuantKernel<T, false><<<grid, block, 0, ctx->stream>>>(p);
+        launchQuant<T, false, WIDE, UNITS>(ctx, p, units);
+    }
+}
+
+template <class T>
+void quantizeAs(Context* ctx, const MxQuantParams& p, bool nv) {
+    // eight columns at a time, all of them there: 16-byte accesses
+    const bool wide = p.cols % 8 == 0 && aligned16(p.src, p.srcLd * sizeof(T)) && (!p.values || aligned16(p.values, p.valuesLd * sizeof(T)));
+    if (!longRows(ctx, p.rows, p.cols / 8)) {
+        wide ? quantizeWith<T, true, 1>(ctx, p, nv) : quantizeWith<T, false, 1>(ctx, p, nv);
+    } else {
+        wide ? quantizeWith<T, true, kUnits>(ctx, p, nv) : quantizeWith<T, false, kUnits>(ctx, p, nv);
+    }
+}
+
+template <class T, int UNITS>
+void dequantizeWith(Context* ctx, const MxDequantParams& p, bool nv) {
+    dim3 grid, block;
+    gridFor(p.rows, (p.cols + 7) / 8, UNITS, &grid, &block);
+    const bool wide = p.cols % 8 == 0 && aligned16(p.out, p.outLd * sizeof(T));
+    if (nv && wide) {
+        mxDequantKernel<T, true, true, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+    } else if (nv) {
+        mxDequantKernel<T, true, false, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+    } else if (wide) {
+        mxDequantKernel<T, false, true, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+    } else {
+        mxDequantKernel<T, false, false, UNITS><<<grid, block, 0, ctx->stream>>>(p);
     }
     B2_CUDA(cudaGetLastError());
     ++ctx->launches;
@@ -302,22 +524,17 @@ void quantizeAs(Context* ctx, const MxQuantParams& p, bool nv) {
 
 template <class T>
 void dequantizeAs(Context* ctx, const MxDequantParams& p, bool nv) {
-    dim3 grid, block;
-    gridFor(ctx, p.rows, (p.cols + 7) / 8, &grid, &block);
-    if (nv) {
-        mxDequantKernel<T, true><<<grid, block, 0, ctx->stream>>>(p);
+    if (!longRows(ctx, p.rows, p.cols / 8)) {
+        dequantizeWith<T, 1>(ctx, p, nv);
     } else {
-        mxDequantKernel<T, false><<<grid, block, 0, ctx->stream>>>(p);
+        dequantizeWith<T, kUnits>(ctx, p, nv);
     }
-    B2_CUDA(cudaGetLastError());
-    ++ctx->launches;
 }
 
 }  // namespace
 
 void launchMxQuantize(Context* ctx, const void* src, int dtype, int64_t srcLd, const b200c_mx_matrix& out, void* values,
                       int64_t valuesLd, bool scaleGiven) {
-    const int es = dtBits(dtype) / 8;
     MxQuantParams p;
     p.src = src;
     p.srcLd = srcLd;
@@ -334,8 +551,6 @@ void launchMxQuantize(Context* ctx, const void* src, int dtype, int64_t srcLd, c
     p.blocks = mxBlocks(out.format, out.cols);
     p.scaleRows = out.cols == 0 ? 0 : p.tiled ? roundUp(out.rows, 128) : out.rows;
     p.scaleBlocks = p.tiled ? roundUp(p.blocks, 4) : p.blocks;
-    p.wideIn = aligned16(src, srcLd * es);
-    p.wideValues = values && aligned16(values, valuesLd * es);
     const bool nv = out.format == B200C_NVFP4;
     if (dtype == B200C_F16) {
         quantizeAs<__half>(ctx, p, nv);
@@ -359,7 +574,6 @@ void launchMxDequantize(Context* ctx, const b200c_mx_matrix& m, void* out, int d
     p.blocks = mxBlocks(m.format, m.cols);
     p.out = out;
     p.outLd = outLd;
-    p.wideOut = aligned16(out, outLd * (dtBits(dtype) / 8));
     const bool nv = m.format == B200C_NVFP4;
     if (dtype == B200C_F16) {
         dequantizeAs<__half>(ctx, p, nv);
