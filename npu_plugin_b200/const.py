@@ -550,20 +550,20 @@ class CudaBackend:
     def mx_quantize(self, src, dtype, src_ld, out, tensor_scale_given=False, values=None, values_ld=0):
         """src (rows x cols of `out`, f16/bf16/f32, src_ld elements between rows) -> the codes and scales of `out`;
         `values` receives what they stand for, in the type of src."""
-        rc = self.lib.b200c_mx_quantize(self.ctx, src, dtype, src_ld, C.byref(out.c), values, values_ld,
+        rc = self.lib.b200c_mx_quantize(self.ctx, src, dtype, src_ld, out.ref, values, values_ld,
                                         A.MX_SCALE_GIVEN if tensor_scale_given and out.c.format == A.NVFP4 else 0)
         if rc:
             raise_for(rc, self._err())
 
     def mx_dequantize(self, m, out, dtype, out_ld):
         """What the codes of `m` stand for -> out (f16/bf16/f32, out_ld elements between rows)."""
-        rc = self.lib.b200c_mx_dequantize(self.ctx, C.byref(m.c), out, dtype, out_ld)
+        rc = self.lib.b200c_mx_dequantize(self.ctx, m.ref, out, dtype, out_ld)
         if rc:
             raise_for(rc, self._err())
 
     def mx_matmul(self, a, b, out, dtype, out_ld):
         """out = a b^T of two matrices with tiled scales (out f16/bf16/f32, out_ld elements between rows)."""
-        rc = self.lib.b200c_mx_matmul(self.ctx, C.byref(a.c), C.byref(b.c), out, dtype, out_ld)
+        rc = self.lib.b200c_mx_matmul(self.ctx, a.ref, b.ref, out, dtype, out_ld)
         if rc:
             raise_for(rc, self._err())
 

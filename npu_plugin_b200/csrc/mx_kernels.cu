@@ -203,6 +203,12 @@ __device__ __forceinline__ float tensorScaleOf(float top) {
 
 constexpr int kUnits = 4;  // units of a thread where rows are long
 
+// See mx_matmul.cu: no kernel here touches memory before the one that was launched before it has ended.
+__device__ __forceinline__ void afterLast() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // How a kernel's threads lie over rows x units (8 elements): x along a row, y over rows, each thread with UNITS
 // units of one row, x apart, whose loads are all under way before the first is used.  Addresses differ by
 // constants between a thread's units: with its units in different rows instead, 64-bit address arithmetic was a
@@ -226,6 +232,7 @@ struct Lay {
 template <class T, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQuantParams p) {
     typedef Lay<UNITS> L;
+    afterLast();
     unsigned int top = 0;
     const int units = static_cast<int>((p.cols + 7) / 8), cols = static_cast<int>(p.cols);
     for (long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; r < p.rows; r += static_cast<long long>(gridDim.x) * blockDim.y) {
@@ -333,6 +340,7 @@ __device__ __forceinline__ unsigned int encode8(const Raw<T>& raw, unsigned int 
 template <class T, bool NV, bool WIDE, bool VALUES, int UNITS>
 __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ MxQuantParams p, int rowCtas) {
     typedef Lay<UNITS> L;
+    afterLast();
     float t = 1.f;
     if (NV) {
         if (p.scaleGiven) {
@@ -395,6 +403,7 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
 template <class T, bool NV, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(256) mxDequantKernel(const __grid_constant__ MxDequantParams p) {
     typedef Lay<UNITS> L;
+    afterLast();
     const float t = NV ? p.tensorScale[0] : 1.f;
     const int cols = static_cast<int>(p.cols), units = (cols + 7) / 8;
     const long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -438,6 +447,21 @@ void gridFor(long long rows, long long units, int unitsOfThread, dim3* grid, dim
                  static_cast<unsigned int>(std::max<long long>(1, std::min<long long>((units + along - 1) / along, 65535))));
 }
 
+template <class Kernel, class... Args>
+void launchNext(Context* ctx, Kernel kernel, dim3 grid, dim3 block, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    ++ctx->launches;
+}
+
 bool aligned16(const void* p, long long ldBytes) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ldBytes % 16 == 0;
 }
@@ -459,12 +483,10 @@ void launchQuant(Context* ctx, const MxQuantParams& p, long long units) {
         grid.x += static_cast<unsigned int>(std::min<long long>((words + perX - 1) / perX, 1024));
     }
     if (p.values) {
-        mxQuantKernel<T, NV, WIDE, true, UNITS><<<grid, block, 0, ctx->stream>>>(p, rowCtas);
+        launchNext(ctx, mxQuantKernel<T, NV, WIDE, true, UNITS>, grid, block, p, rowCtas);
     } else {
-        mxQuantKernel<T, NV, WIDE, false, UNITS><<<grid, block, 0, ctx->stream>>>(p, rowCtas);
+        launchNext(ctx, mxQuantKernel<T, NV, WIDE, false, UNITS>, grid, block, p, rowCtas);
     }
-    B2_CUDA(cudaGetLastError());
-    ++ctx->launches;
 }
 
 template <class T, bool WIDE, int UNITS>
@@ -472,9 +494,7 @@ void launchTop(Context* ctx, const MxQuantParams& p) {
     dim3 grid, block;
     gridFor(p.rows, (p.cols + 7) / 8, UNITS, &grid, &block);
     grid.x = std::min<unsigned int>(grid.x, ctx->smCount * 16u);  // few warps end with an atomic
-    mxTopKernel<T, WIDE, UNITS><<<grid, block, 0, ctx->stream>>>(p);
-    B2_CUDA(cudaGetLastError());
-    ++ctx->launches;
+    launchNext(ctx, mxTopKernel<T, WIDE, UNITS>, grid, block, p);
 }
 
 template <class T, bool WIDE, int UNITS>
@@ -510,16 +530,14 @@ void dequantizeWith(Context* ctx, const MxDequantParams& p, bool nv) {
     gridFor(p.rows, (p.cols + 7) / 8, UNITS, &grid, &block);
     const bool wide = p.cols % 8 == 0 && aligned16(p.out, p.outLd * sizeof(T));
     if (nv && wide) {
-        mxDequantKernel<T, true, true, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+        launchNext(ctx, mxDequantKernel<T, true, true, UNITS>, grid, block, p);
     } else if (nv) {
-        mxDequantKernel<T, true, false, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+        launchNext(ctx, mxDequantKernel<T, true, false, UNITS>, grid, block, p);
     } else if (wide) {
-        mxDequantKernel<T, false, true, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+        launchNext(ctx, mxDequantKernel<T, false, true, UNITS>, grid, block, p);
     } else {
-        mxDequantKernel<T, false, false, UNITS><<<grid, block, 0, ctx->stream>>>(p);
+        launchNext(ctx, mxDequantKernel<T, false, false, UNITS>, grid, block, p);
     }
-    B2_CUDA(cudaGetLastError());
-    ++ctx->launches;
 }
 
 template <class T>

@@ -50,9 +50,9 @@ struct Tile {
     static constexpr int chunksPerTile = NV ? 4 : 2;  // 512-byte tiles of scales per stage and 128 rows
     static constexpr int bytesP = 128 * 128;
     static constexpr int bytesQ = BN * 128;
-    static constexpr int scaleBytes = chunksPerTile * 512;  // of each side: no tile of Q crosses 128 rows
+    static constexpr int scaleBytes = chunksPerTile * 512;  // of each side: a tile of Q begins where 128 rows do
     static constexpr int stageBytes = (bytesP + bytesQ + 2 * scaleBytes + 1023) / 1024 * 1024;
-    static constexpr int stages = BN <= 32 ? 4 : 3;         // two CTAs fit an SM
+    static constexpr int stages = BN <= 16 ? 5 : BN <= 32 ? 4 : 3;         // two CTAs fit an SM
     static constexpr int smemBytes = 1024 /* alignment */ + stages * stageBytes;
     static constexpr int scaleCols = 2 * chunksPerTile * 4;  // tensor memory columns of a stage's scales
     static constexpr int scaleBufs = 2;
@@ -69,8 +69,9 @@ struct PairTile {
     static constexpr int bytesSide = 128 * 128;
     static constexpr int scaleBytes = chunksPerTile * 512;  // of 128 rows
     static constexpr int stageBytes = (2 * bytesSide + 3 * scaleBytes + 1023) / 1024 * 1024;
-    static constexpr int stages = NV ? 5 : 6;
-    static constexpr int smemBytes = 1024 + stages * stageBytes;
+    static constexpr int stages = 5;
+    static constexpr int stagingBytes = 2 * 32 * 128;  // of an epilogue warp: two groups of 32 x 32 values on their way out
+    static constexpr int smemBytes = 1024 + stages * stageBytes + 4 * stagingBytes;
     static constexpr int accStep = 160, scaleCol = 416;
     static constexpr int scaleCols = 3 * chunksPerTile * 4;
     static constexpr int scaleBufs = 96 / scaleCols;
@@ -109,6 +110,19 @@ __device__ __noinline__ bool barWaitSlow(unsigned int bar, unsigned int parity, 
 __device__ __forceinline__ bool barWait(unsigned int bar, unsigned int parity, volatile int* stalled) {
     if (barTry(bar, parity)) return true;
     return barWaitSlow(bar, parity, stalled);
+}
+
+// The kernels here and those of mx_kernels.cu are launched so that the next one's CTAs may start while the last
+// ones of this are at work (programmatic stream serialisation): nothing that another kernel wrote or reads is
+// touched, and no tensor memory taken, before afterLast(); allowNext() comes behind the CTA's own allocation.
+__device__ __forceinline__ void afterLast() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void allowNext() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void prefetchMap(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 // One thread of the warp, the same one every time and known to the compiler as such: the operands of
@@ -237,19 +251,36 @@ __device__ __forceinline__ void mmaStage(unsigned int acc, unsigned long long dp
     }
 }
 
-__device__ __forceinline__ void readColumns(unsigned int addr, float v[32]) {
-    unsigned int r[32];
+// 32 columns of this warp's lanes; the values are there after readsDone()
+__device__ __forceinline__ void startRead(unsigned int addr, unsigned int r[32]) {
     asm volatile(
             "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
             "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-            "tcgen05.wait::ld.sync.aligned;"
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
             : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
               "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
               "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
               "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
             : "r"(addr)
             : "memory");
+}
+// ties the registers of a read to the wait, so that nothing uses them before it
+__device__ __forceinline__ void readsDone(unsigned int r[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+    asm volatile(""
+                 : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void readColumns(unsigned int addr, float v[32]) {
+    unsigned int r[32];
+    startRead(addr, r);
+    readsDone(r);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -328,22 +359,74 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
     }
 }
 
-// The tile's sums lie in `split` CTAs' shared memory as [BN][128]; this CTA adds up its share of the columns, in
-// the order of the ranks.
-template <class T, int BN>
-__device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int row, long long p, long long q0,
-                                            float alpha) {
+// The tile's sums lie in `split` (at most MOST) CTAs' shared memory as [BN][128]; this CTA adds up its share of the
+// columns, in the order of the ranks.  A thread takes four rows at a time, and 16 loads from the cluster's memory
+// are under way at once: with one column at a time the waiting for them took longer than the product itself.
+template <class T, int BN, int MOST>
+__device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0,
+                                            long long q0, float alpha) {
+    constexpr int most = 16 / MOST;
     const int c0 = static_cast<int>(rank) * BN / g.split, c1 = (static_cast<int>(rank) + 1) * BN / g.split;
-    for (int c = c0; c < c1; ++c) {
-        if (q0 + c >= g.rowsQ) break;
-        float v = 0.f;
-        for (int r = 0; r < g.split; ++r) {
-            float w;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(addrIn(sums + (c * 128 + row) * 4, r)) : "memory");
-            v = v + w;
+    const int row = thread % 32 * 4;
+    const long long p = p0 + row;
+    const int rows = static_cast<int>(min(4ll, g.rowsP - p)), cols = static_cast<int>(min(static_cast<long long>(c1), g.rowsQ - q0));
+    if (rows <= 0) return;
+    unsigned int from[MOST];
+#pragma unroll
+    for (int r = 0; r < MOST; ++r) from[r] = addrIn(sums + row * 4, min(r, g.split - 1));
+    for (int c = c0 + thread / 32; c < cols; c += 4 * most) {
+        float w[most][MOST][4];
+#pragma unroll
+        for (int j = 0; j < most; ++j) {
+#pragma unroll
+            for (int r = 0; r < MOST; ++r) {
+                if (r < g.split && c + 4 * j < cols) {
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(w[j][r][0]), "=f"(w[j][r][1]), "=f"(w[j][r][2]), "=f"(w[j][r][3])
+                                 : "r"(from[r] + (c + 4 * j) * 512)
+                                 : "memory");
+                }
+            }
         }
-        const float one[1] = {v * alpha};
-        storeColumns<T, 1>(g, p, q0 + c, one);
+#pragma unroll
+        for (int j = 0; j < most; ++j) {
+            const long long q = q0 + c + 4 * j;
+            if (c + 4 * j >= cols) break;
+            alignas(16) T v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float s = w[j][0][i];
+#pragma unroll
+                for (int r = 1; r < MOST; ++r)
+                    if (r < g.split) s = s + w[j][r][i];
+                v[i] = toOut<T>(s * alpha);
+            }
+            T* out = static_cast<T*>(g.out);
+            if (g.across && g.wide && rows == 4) {
+                T* at = out + q * g.ld + p;
+                if (sizeof(T) == 4) {
+                    *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(v);
+                } else {
+                    *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(v);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < rows) out[g.across ? q * g.ld + p + i : (p + i) * g.ld + q] = v[i];
+            }
+        }
+    }
+}
+
+template <class T, int BN>
+__device__ __forceinline__ void join(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0, long long q0,
+                                     float alpha) {
+    if (g.split <= 2) {
+        joinColumns<T, BN, 2>(g, sums, rank, thread, p0, q0, alpha);
+    } else if (g.split <= 4) {
+        joinColumns<T, BN, 4>(g, sums, rank, thread, p0, q0, alpha);
+    } else {
+        joinColumns<T, BN, 8>(g, sums, rank, thread, p0, q0, alpha);
     }
 }
 
@@ -367,6 +450,8 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     const int n = static_cast<int>(static_cast<long long>(g.ktiles) * (rank + 1) / g.split) - k0;
 
     if (threadIdx.x == 0) {
+        prefetchMap(&mapP);
+        prefetchMap(&mapQ);
         for (int s = 0; s < S::stages; ++s) {
             barInit(full + 8 * s, 1);
             barInit(empty + 8 * s, 1);
@@ -375,6 +460,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         stalledWord = 0;
     }
+    afterLast();
     if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&tmemBase)), "r"(S::cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -382,6 +468,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    allowNext();
     const unsigned int acc = tmemBase, scaleCol = tmemBase + BN;
 
     if (warp == 4) {
@@ -411,8 +498,6 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     } else if (warp == 5) {
         const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesP);
         const unsigned long long ds0 = scaleDesc(stage0 + S::bytesP + S::bytesQ);
-        // rows of a Q tile that starts inside 128 rows: the scales of 32 rows are one column of a word's four
-        const unsigned int shiftQ = static_cast<unsigned int>(q0 % 128) / 32;
         int s = 0, phase = 0;
         for (int i = 0; i < n; ++i) {
             bool ok = barWait(full + 8 * s, phase, stalled);
@@ -434,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
                         copyScales(colQ + c * 4, ds0 + off + S::scaleBytes / 16 + c * 32);
                     }
                 }
-                mmaStage<128, BN, NV, false>(acc, dp0 + off, dq0 + off, colP, colQ + shiftQ, 4, steps, i == 0);
+                mmaStage<128, BN, NV, false>(acc, dp0 + off, dq0 + off, colP, colQ, 4, steps, i == 0);
                 mmaCommit(empty + 8 * s);
                 if (i + 1 == n) mmaCommit(done);
             }
@@ -479,11 +564,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         clusterSync();
         if (finished) {
             if (g.outTag == T_F16) {
-                joinColumns<__half, BN>(g, stage0, rank, row, p0 + row, q0, alpha);
+                join<__half, BN>(g, stage0, rank, row, p0, q0, alpha);
             } else if (g.outTag == T_BF16) {
-                joinColumns<__nv_bfloat16, BN>(g, stage0, rank, row, p0 + row, q0, alpha);
+                join<__nv_bfloat16, BN>(g, stage0, rank, row, p0, q0, alpha);
             } else {
-                joinColumns<float, BN>(g, stage0, rank, row, p0 + row, q0, alpha);
+                join<float, BN>(g, stage0, rank, row, p0, q0, alpha);
             }
         }
         __syncwarp();
@@ -508,30 +593,66 @@ __device__ __forceinline__ void tileOf(const MxMatmulParams& g, int t, int* p, i
     *p = group * G + (r - *q * high);
 }
 
+// 32 columns of a warp's 32 rows -> the product, through shared memory and a bulk store: a row's 32 values are
+// 64 or 128 bytes, which leave together, where a thread's own stores of its row would be 16 bytes of 32
+// different rows at a time.
 template <class T>
-__device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, unsigned int acc, int buf, long long p, long long q0, float alpha,
-                                             unsigned int accFree, int lane) {
+__device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtensorMap* mapOut, unsigned int staging, int group, int lane,
+                                           long long row0, long long col0, const unsigned int r[32], float alpha) {
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * alpha;
+    if (!g.wide) {
+        storeColumns<T, 32>(g, row0 + lane, col0, v);
+        return;
+    }
+    constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16;
+    const unsigned int at = staging + (group & 1) * 32 * 128;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the store before the last has read its half
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < chunks; ++c) {
+        alignas(16) T t[16 / sizeof(T)];
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(16 / sizeof(T)); ++j) t[j] = toOut<T>(v[c * (16 / sizeof(T)) + j]);
+        const uint4 w = *reinterpret_cast<const uint4*>(t);
+        // the map's swizzle: 16-byte chunks of a row of 64 or 128 bytes change places with the row's number
+        const unsigned int to = at + lane * rowBytes + ((c ^ (chunks == 8 ? lane & 7 : (lane >> 1) & 3)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        if (row0 < g.rowsP && col0 < g.rowsQ) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(mapOut),
+                         "r"(static_cast<int>(col0)), "r"(static_cast<int>(row0)), "r"(at)
+                         : "memory");
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, const CUtensorMap* mapOut, unsigned int staging, unsigned int acc, int buf,
+                                             long long row0, long long q0, float alpha, unsigned int accFree, int lane) {
     // columns 160..255 of tensor memory belong to both buffers: they are read first, and the next tile may start
     const int shared0 = buf ? 0 : 160;
-    float v[3][32];
+    unsigned int r[3][32];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) readColumns(acc + shared0 + i * 32, v[i]);
+    for (int i = 0; i < 3; ++i) startRead(acc + shared0 + i * 32, r[i]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) readsDone(r[i]);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(accFree) : "memory");
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[i][j] = v[i][j] * alpha;
-        storeColumns<T, 32>(g, p, q0 + shared0 + i * 32, v[i]);
-    }
+    for (int i = 0; i < 3; ++i) storeGroup<T>(g, mapOut, staging, i, lane, row0, q0 + shared0 + i * 32, r[i], alpha);
     const int rest = buf ? 96 : 0;
 #pragma unroll 1
-    for (int c = 0; c < 160; c += 32) {
-        readColumns(acc + rest + c, v[0]);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[0][j] = v[0][j] * alpha;
-        storeColumns<T, 32>(g, p, q0 + rest + c, v[0]);
+    for (int i = 0; i < 5; ++i) {
+        startRead(acc + rest + i * 32, r[0]);
+        readsDone(r[0]);
+        storeGroup<T>(g, mapOut, staging, i + 3, lane, row0, q0 + rest + i * 32, r[0], alpha);
     }
 }
 
@@ -539,6 +660,7 @@ template <bool NV>
 __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_constant__ CUtensorMap mapP, const __grid_constant__ CUtensorMap mapQ,
                                                                const __grid_constant__ CUtensorMap mapScalesP,
                                                                const __grid_constant__ CUtensorMap mapScalesQ,
+                                                               const __grid_constant__ CUtensorMap mapOut,
                                                                const __grid_constant__ MxMatmulParams g) {
     typedef PairTile<NV> S;
     extern __shared__ unsigned char raw[];
@@ -553,6 +675,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
     const int tiles = g.tilesP * g.tilesQ, pairs = gridDim.x / 2;
 
     if (threadIdx.x == 0) {
+        prefetchMap(&mapP);
+        prefetchMap(&mapQ);
+        prefetchMap(&mapScalesP);
+        prefetchMap(&mapScalesQ);
+        if (g.wide) prefetchMap(&mapOut);
         for (int s = 0; s < S::stages; ++s) {
             barInit(full + 8 * s, 1);
             barInit(empty + 8 * s, 1);
@@ -562,6 +689,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         stalledWord = 0;
     }
+    afterLast();
     if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemAddr(&tmemBase)), "r"(S::cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -570,6 +698,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
     __syncthreads();
     clusterSync();  // both CTAs' barriers are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    allowNext();
     const unsigned int tmem = tmemBase;
 
     if (warp == 4) {
@@ -636,6 +765,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
     } else if (warp < 4) {
         const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
         const unsigned int accFree0 = addrIn(accFree, 0);
+        const unsigned int staging = stage0 + S::stages * S::stageBytes + warp * S::stagingBytes;
         int done = 0;
         for (int t = blockIdx.x / 2; t < tiles; t += pairs, ++done) {
             int tp, tq;
@@ -644,16 +774,17 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int buf = done & 1;
             const unsigned int acc = tmem + buf * S::accStep + (static_cast<unsigned int>(warp * 32) << 16);
-            const long long p = static_cast<long long>(tp) * 256 + rank * 128 + warp * 32 + lane, q0 = static_cast<long long>(tq) * 256;
+            const long long row0 = static_cast<long long>(tp) * 256 + rank * 128 + warp * 32, q0 = static_cast<long long>(tq) * 256;
             if (g.outTag == T_F16) {
-                pairEpilogue<__half>(g, acc, buf, p, q0, alpha, accFree0, lane);
+                pairEpilogue<__half>(g, &mapOut, staging, acc, buf, row0, q0, alpha, accFree0, lane);
             } else if (g.outTag == T_BF16) {
-                pairEpilogue<__nv_bfloat16>(g, acc, buf, p, q0, alpha, accFree0, lane);
+                pairEpilogue<__nv_bfloat16>(g, &mapOut, staging, acc, buf, row0, q0, alpha, accFree0, lane);
             } else {
-                pairEpilogue<float>(g, acc, buf, p, q0, alpha, accFree0, lane);
+                pairEpilogue<float>(g, &mapOut, staging, acc, buf, row0, q0, alpha, accFree0, lane);
             }
         }
     }
+    if (warp < 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the last stores are through
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     clusterSync();  // neither CTA leaves while the other's products, copies or arrivals reach into it
@@ -709,6 +840,24 @@ CUtensorMap scaleMapOf(const b200c_mx_matrix& m, int chunksPerTile, int boxTiles
     return map;
 }
 
+// The product as groups of 32 x 32 values; what lies behind its last row or column is not written.
+CUtensorMap outMapOf(void* out, int dtype, int64_t rows, int64_t cols, int64_t ld) {
+    CUtensorMap map;
+    const int es = dtBits(dtype) / 8;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * es)};
+    const cuuint32_t box[2] = {32, 32};
+    const cuuint32_t step[2] = {1, 1};
+    const CUtensorMapDataType type = dtype == B200C_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : dtype == B200C_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    const CUresult r = encodeTiled()(&map, type, 2, out, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                     es == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw CudaFail("cuTensorMapEncodeTiled failed with " + std::to_string(static_cast<int>(r)));
+    return map;
+}
+
 // The kernel may use `bytes` of shared memory; told once per device.
 template <class Kernel>
 void allowSmem(Context* ctx, Kernel kernel, int bytes, std::atomic<unsigned long long>& ready) {
@@ -726,14 +875,36 @@ void launchClusters(Context* ctx, void (*kernel)(Args...), unsigned int ctas, un
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = perCluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = perCluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = perCluster > 1 ? 2 : 1;
     B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     ++ctx->launches;
+}
+
+// How many CTAs share a tile's k.  In us: a stage takes about 0.34 where its loads are waited for, the CTAs that do
+// not fit the SMs one by one follow or share an SM, and joining the sums costs more the more there are of
+// them.  Measured for 1 x 11008 x 4096 with 1, 2, 3, 4 CTAs: 7.6, 7.2, 6.6, 9.4; 16 x 4096 x 11008 with 1, 2, 4, 8:
+// 15.7, 10.1, 6.6, 7.2; 128 x 4096 x 4096: 8.8, 8.2, 7.2, 10.2; 77 x 515 x 1003: 4.7, 6.3, 5.5.
+int splitOf(Context* ctx, long long tiles, int ktiles, int bn) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 8 && s <= ktiles; ++s) {
+        const long long rounds = (tiles * s + ctx->smCount - 1) / ctx->smCount;
+        if (s > 1 && rounds > (bn <= 32 ? 2 : 1)) break;
+        const double cost = 0.34 * static_cast<double>(rounds * ((ktiles + s - 1) / s)) * (rounds > 1 ? 0.9 : 1.0) +
+                            (s > 1 ? 0.3 + 0.011 * bn + 0.05 * s : 0.0);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
 }
 
 template <int BN, bool NV>
@@ -744,16 +915,14 @@ void launchTileOf(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix&
     g.tilesP = static_cast<int>((p.rows + 127) / 128);
     g.tilesQ = static_cast<int>((q.rows + BN - 1) / BN);
     const long long tiles = static_cast<long long>(g.tilesP) * g.tilesQ;
-    // two CTAs per SM: k is shared out while there are CTAs to spare and each keeps two stages' worth
-    g.split = 1;
-    while (g.split < 8 && tiles * g.split * 2 <= 2 * ctx->smCount && g.ktiles >= 4 * g.split) g.split *= 2;
+    g.split = splitOf(ctx, tiles, g.ktiles, BN);
     if (tiles * g.split > 0x7FFFFFFFll) throw BadArg("the product has too many tiles");
     launchClusters(ctx, mxMatmulKernel<BN, NV>, static_cast<unsigned int>(tiles * g.split), static_cast<unsigned int>(g.split), S::smemBytes,
                    mapOf(p, 128), mapOf(q, BN), g);
 }
 
 template <bool NV>
-void launchPairs(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix& q, MxMatmulParams g) {
+void launchPairs(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix& q, int dtype, MxMatmulParams g) {
     typedef PairTile<NV> S;
     static std::atomic<unsigned long long> ready{0};
     allowSmem(ctx, mxMatmulPairKernel<NV>, S::smemBytes, ready);
@@ -763,7 +932,8 @@ void launchPairs(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix& 
     if (tiles > 0x3FFFFFFFll) throw BadArg("the product has too many tiles");
     const long long pairs = std::min<long long>(tiles, ctx->smCount / 2);
     launchClusters(ctx, mxMatmulPairKernel<NV>, static_cast<unsigned int>(2 * pairs), 2u, S::smemBytes, mapOf(p, 128), mapOf(q, 128),
-                   scaleMapOf(p, S::chunksPerTile, 1), scaleMapOf(q, S::chunksPerTile, 2), g);
+                   scaleMapOf(p, S::chunksPerTile, 1), scaleMapOf(q, S::chunksPerTile, 2),
+                   g.wide ? outMapOf(g.out, dtype, p.rows, q.rows, g.ld) : CUtensorMap{}, g);
 }
 
 template <int BN>
@@ -813,9 +983,9 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     g.err = ctx->errWord;
     if (pairs) {
         if (nv) {
-            launchPairs<true>(ctx, p, q, g);
+            launchPairs<true>(ctx, p, q, dtype, g);
         } else {
-            launchPairs<false>(ctx, p, q, g);
+            launchPairs<false>(ctx, p, q, dtype, g);
         }
     } else if (q.rows <= 16) {
         launchFormat<16>(ctx, p, q, g);

@@ -24,6 +24,7 @@ class MxMatrix:
         if ld is None:
             ld = sizes(fmt, rows, cols, layout)[0]
         self.c = A.b200c_mx_matrix(fmt, layout, rows, cols, ld, codes, scales, tensor_scale)
+        self.ref = C.byref(self.c)
 
     @property
     def shape(self):
