@@ -606,9 +606,9 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
         storeColumns<T, 32>(g, row0 + lane, col0, v);
         return;
     }
-    constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16;
-    const unsigned int at = staging + (group & 1) * 32 * 128;
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the store before the last has read its half
+    constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16, bufs = 2 * 128 / rowBytes;
+    const unsigned int at = staging + (group % bufs) * 32 * rowBytes;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(bufs - 1) : "memory");  // the last store from here has been read
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < chunks; ++c) {
@@ -644,7 +644,7 @@ __device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, const CUte
     for (int i = 0; i < 3; ++i) readsDone(r[i]);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncwarp();
-    if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(accFree) : "memory");
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(accFree) : "memory");
 #pragma unroll
     for (int i = 0; i < 3; ++i) storeGroup<T>(g, mapOut, staging, i, lane, row0, q0 + shared0 + i * 32, r[i], alpha);
     const int rest = buf ? 96 : 0;
@@ -728,37 +728,40 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
         if (*stalled && rank == 0) {  // copies in flight write both CTAs' memory, which stays until they have
             for (int i = max(0, issued - S::stages); i < issued; ++i) drain(full + 8 * (i % S::stages), (i / S::stages) & 1);
         }
-    } else if (warp == 5 && rank == 0) {
+    } else if (warp == 5 && rank == 0 && electOne()) {
         const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesSide);
         const unsigned long long ds0 = scaleDesc(stage0 + 2 * S::bytesSide);
         int s = 0, phase = 0, it = 0, done = 0;
+        int before = 0, beforePhase = 0;  // the stage, scaleBufs ago, whose products must be done with their scales
         bool ok = true;
         for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs, ++done) {
             const unsigned int acc = tmem + (done & 1) * S::accStep;
-            if (done > 0) ok = __all_sync(0xFFFFFFFFu, barWait(accFree, (done - 1) & 1, stalled));
+            if (done > 0) ok = barWait(accFree, (done - 1) & 1, stalled);
             for (int kt = 0; kt < g.ktiles && ok; ++kt, ++it) {
                 ok = barWait(full + 8 * s, phase, stalled);
                 // as above: a copy of scales waits for the products that read the columns before
-                if (it >= S::scaleBufs) ok = ok && barWait(empty + 8 * ((it - S::scaleBufs) % S::stages), ((it - S::scaleBufs) / S::stages) & 1, stalled);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (it >= S::scaleBufs) {
+                    ok = ok && barWait(empty + 8 * before, beforePhase, stalled);
+                    if (++before == S::stages) before = 0, beforePhase ^= 1;
+                }
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (electOne()) {
-                    const unsigned int colP = tmem + S::scaleCol + (it % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
-                    const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
-                    const int steps = kt + 1 < g.ktiles ? kTileK / kStepK
-                                                        : static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+                const unsigned int colP = tmem + S::scaleCol + (it % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
+                const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
 #pragma unroll
-                    for (int c = 0; c < S::chunksPerTile; ++c) {
-                        copyScalesPair(colP + c * 4, ds0 + off + c * 32);
-                        copyScalesPair(colQ + c * 8, ds0 + off + S::scaleBytes / 16 + c * 32);
-                        copyScalesPair(colQ + c * 8 + 4, ds0 + off + S::scaleBytes / 8 + c * 32);
-                    }
-                    mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, steps, kt == 0);
-                    mmaCommitPair(empty + 8 * s);
-                    if (kt + 1 == g.ktiles) mmaCommitPair(accFull);
+                for (int c = 0; c < S::chunksPerTile; ++c) {
+                    copyScalesPair(colP + c * 4, ds0 + off + c * 32);
+                    copyScalesPair(colQ + c * 8, ds0 + off + S::scaleBytes / 16 + c * 32);
+                    copyScalesPair(colQ + c * 8 + 4, ds0 + off + S::scaleBytes / 8 + c * 32);
                 }
-                __syncwarp();
+                if (kt + 1 < g.ktiles) {
+                    mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, kTileK / kStepK, kt == 0);
+                } else {
+                    const int steps = static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+                    mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, steps, kt == 0);
+                }
+                mmaCommitPair(empty + 8 * s);
+                if (kt + 1 == g.ktiles) mmaCommitPair(accFull);
                 if (++s == S::stages) s = 0, phase ^= 1;
             }
         }
