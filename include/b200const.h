@@ -137,7 +137,19 @@ enum b200c_xform_kind {
      * side0 / side1 receive the per-channel f32 scales / i32 zero points
      * (same residency as the fold output).  The result holds the integral
      * values in f32 storage; follow it with ConvertElemType + QuantCast.      */
-    B200C_X_QUANTIZE_SYNTH = 100
+    B200C_X_QUANTIZE_SYNTH = 100,
+    /* Block-scaled 4-bit quantisation of a float tensor (f16, bf16, f32), no reference counterpart; see
+     * "block-scaled 4-bit matrices" below.  i0 = format, f = the tensor scale of B200C_NVFP4 (0: the one
+     * that the data gives).  The rows are those of the memory order: its innermost dimension, which has
+     * to be a multiple of 32 elements (PadWithZero in front of it makes it one).  The element type becomes
+     * B200C_F4E2M1; only SwizzleConstant and DequantizeMx may follow.  side0 receives the scales
+     * (B200C_MX_SCALES_ROWS), side1 the two floats of the tensor scale (B200C_NVFP4); either may be NULL.
+     * Residency as the fold output.                                                   */
+    B200C_X_QUANTIZE_MX = 101,
+    /* Its inverse: content of type B200C_F4E2M1 -> type.dtype (f16, bf16 or f32).  i0 = format; side0 = the
+     * scales, side1 = the tensor scale (B200C_NVFP4), which are read here: with the residency of the fold
+     * output, or NULL right behind a QuantizeMx, whose own are taken then.                  */
+    B200C_X_DEQUANTIZE_MX = 102
 };
 
 #define B200C_QSYNTH_SYM_I8 0

@@ -53,6 +53,8 @@ X_REVERSE = 17
 X_EXPAND_DILATED = 18
 X_RELOCATE_WEIGHTS_TABLE = 19
 X_QUANTIZE_SYNTH = 100
+X_QUANTIZE_MX = 101
+X_DEQUANTIZE_MX = 102
 
 QSYNTH_SYM_I8, QSYNTH_ASYM_U4 = 0, 1
 

@@ -72,6 +72,9 @@ class ShardFolder:
         self.folded_offsets, self.folded_sizes = [], []
         at = 0
         for d in decls:
+            if any(t.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX) and isinstance(s, np.ndarray) for t in d.transforms
+                   for s in (t.side0, t.side1)):
+                raise ValueError(f"{d.name}: scales of a constant that is folded on the device have to lie there")
             final = backend.infer_type(d.base_type, d.transforms)
             size = final.getTotalAllocSize()
             bt = d.base_type.to_c(self._keep)
@@ -125,7 +128,7 @@ class ShardFolder:
                 if side_ptrs is not None and side_ptrs[i] is not None:
                     ch = self._prepared[i][1]
                     for k in range(self._prepared[i][2]):
-                        if ch[k].kind == A.X_QUANTIZE_SYNTH:
+                        if ch[k].kind in (A.X_QUANTIZE_SYNTH, A.X_QUANTIZE_MX):
                             ch[k].side0, ch[k].side1 = side_ptrs[i]
             self._marshalled = key
         for first, last in self._groups(max_batch_bytes):
@@ -165,7 +168,7 @@ class ShardFolder:
             self._marshalled = None
             if side_ptrs is not None and side_ptrs[i] is not None:
                 for k in range(n):
-                    if ch[k].kind == A.X_QUANTIZE_SYNTH:
+                    if ch[k].kind in (A.X_QUANTIZE_SYNTH, A.X_QUANTIZE_MX):
                         ch[k].side0, ch[k].side1 = side_ptrs[i]
             rc = lib.b200c_fold(ctx, C.byref(bt), data_ptrs[i], d.nbytes, int(d.is_splat), int(data_on_device), ch, n,
                                 folded_ptr + self.folded_offsets[i], self.folded_sizes[i], 1, C.byref(self._nb), None,

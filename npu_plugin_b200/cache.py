@@ -217,6 +217,8 @@ def storage_dtype_after(base_dtype, transforms, infer):
             storage = infer(k + 1).dtype
         elif t.kind == A.X_RELOCATE_WEIGHTS_TABLE:
             storage = A.SI32
+        elif t.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX):
+            storage = infer(k + 1).dtype
     return storage
 
 

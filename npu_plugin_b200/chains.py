@@ -10,12 +10,14 @@ of this convolution" instead of hand-assembling the list.
   flatten_sparse_weights       compressConstWeightsType, src/vpux_compiler/src/dialect/VPUIP/passes/flatten_sparse_weights_types.cpp:41-73
   sparse_identity_filter       createFilter, src/vpux_compiler/src/dialect/VPU/transforms/passes/lower_sparsity_ops.cpp:209-250
   hwtest_default_weights       generateDefaultWeightsAttr, src/vpux_translate_utils/src/hwtest/hwtest_utils.cpp:184-197
+  mx_weights                   (no counterpart: the narrowest weights of the reference are int4 with a scale per channel)
   attach_swizzle               Swizzling::attachSwizzleTransformation, src/vpux_compiler/src/dialect/VPUIP/passes/swizzling.cpp:469-500
 """
 import numpy as np
 
 from . import _cabi as A
 from .const import ContentAttr, DimsOrder, NDType, Quant, Transform
+from .mx import MxMatrix, sizes as mx_sizes
 
 VPU_WEIGHT_SET_BYTE_ALIGNMENT = 16  # nce_invariant.hpp:39
 SWIZZLING_KEY_5 = 5
@@ -117,6 +119,59 @@ def hwtest_default_weights(weights, quant=None):
         if A.dtype_bits(quant.storage) == 4:
             a = a.bitPack(4)
     return a
+
+
+def mx_weights(weights, activations, outputs, tolerance, formats=(A.NVFP4, A.MXFP4)):
+    """The weights of a linear layer in block-scaled 4 bits, if the layer can bear it: `activations` [tokens, inputs] and
+    `outputs` [tokens, rows] are what went into the layer and came out of it in a calibration run (bias left
+    out).  For each of `formats` in turn the folded weights and the activations are quantised, multiplied and compared with
+    the outputs; the first whose error -- 2-norm of the difference over 2-norm of the outputs -- is at most `tolerance`
+    is taken: returns (weights.quantizeMx(format), format, error).  Otherwise (weights, None, smallest error), and the layer keeps what it
+    had.  The weights' rows are those of quantizeMx: all dimensions but the innermost one in memory."""
+    backend = weights._backend
+    t = weights.getType()
+    cols = t.getMemShape()[-1]
+    rows = t.getNumElements() // cols if cols else 0
+    x = np.ascontiguousarray(activations)
+    want = np.asarray(outputs, np.float64)
+    if x.ndim != 2 or x.shape[1] != cols or want.shape != (x.shape[0], rows) or 0 in want.shape + x.shape:
+        raise ValueError(f"mx_weights: {rows} x {cols} weights, activations {x.shape}, outputs {want.shape}")
+    if x.dtype not in (np.float16, np.float32):
+        raise ValueError("mx_weights: activations have to be float16 or float32")
+    xtype = A.F16 if x.dtype == np.float16 else A.F32
+    scale = float(np.linalg.norm(want))
+    least = float("inf")
+    for fmt in formats:
+        weights.quantizeMx(fmt)  # what quantizeMx refuses is refused before anything runs
+    held = []
+
+    def room(nbytes):
+        held.append(backend.dev_alloc(nbytes))
+        return held[-1]
+
+    folded = backend.fold_resident(weights._baseType, weights._base, weights._isSplat, weights.getTransformations())
+    try:
+        dx, dout = room(x.nbytes), room(want.size * 4)
+        backend.upload(dx, x)
+        for fmt in formats:
+            sides = []
+            for src, dtype, n in ((dx, xtype, x.shape[0]), (folded.buf, t.dtype, rows)):
+                ld, codes, scales = mx_sizes(fmt, n, cols)
+                m = MxMatrix(fmt, n, cols, room(codes), room(scales), room(8), ld=ld)
+                backend.mx_quantize(src, dtype, cols, m)
+                sides.append(m)
+            backend.mx_matmul(sides[0], sides[1], dout, A.F32, rows)
+            backend.synchronize()
+            got = backend.download(dout, want.size * 4).view(np.float32).reshape(want.shape).astype(np.float64)
+            error = float(np.linalg.norm(got - want)) / scale if scale else float(np.linalg.norm(got))
+            least = min(least, error)
+            if error <= tolerance:
+                return weights.quantizeMx(fmt), fmt, error
+    finally:
+        folded.release()
+        for p in held:
+            backend.dev_free(p)
+    return weights, None, least
 
 
 def attach_swizzle(attr, key=SWIZZLING_KEY_5, arch=ARCH_VPUX37XX):

@@ -213,7 +213,7 @@ _NAMES = {A.X_CONVERT_ELEM_TYPE: "ConvertElemType", A.X_QUANT_CAST: "QuantCast",
           A.X_SPARSIFY: "Sparsify", A.X_SWIZZLE_CONSTANT: "SwizzleConstant", A.X_RESHAPE: "Reshape",
           A.X_CHANGE_SHAPE_AND_ELEM_TYPE: "ChangeShapeAndElemType", A.X_BROADCAST: "Broadcast",
           A.X_TRANSPOSE: "Transpose", A.X_REVERSE: "Reverse", A.X_EXPAND_DILATED: "ExpandDilated", A.X_RELOCATE_WEIGHTS_TABLE: "RelocateWeightsTable",
-          A.X_QUANTIZE_SYNTH: "QuantizeSynth"}
+          A.X_QUANTIZE_SYNTH: "QuantizeSynth", A.X_QUANTIZE_MX: "QuantizeMx", A.X_DEQUANTIZE_MX: "DequantizeMx"}
 
 
 class Transform:
@@ -230,7 +230,10 @@ class Transform:
         """Value identity of the transformation (MLIR attributes are uniqued by value)."""
         e = self.elem
         ek = (e.kind, e.storage, e.expressed, tuple(e.scales), tuple(e.zps), e.axis, e.qmin, e.qmax) if isinstance(e, Quant) else e
-        return (self.kind, self.a, self.b, self.f, self.i0, self.i1, ek, None if self.aux is None else tuple(self.aux))
+        # the scales that QuantizeMx writes and DequantizeMx reads belong to the transformation, as a base content does
+        # to its attribute: two with scales of their own are not one
+        mine = (id(self.side0), id(self.side1)) if self.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX) else ()
+        return (self.kind, self.a, self.b, self.f, self.i0, self.i1, ek, None if self.aux is None else tuple(self.aux)) + mine
 
     def __eq__(self, o):
         return isinstance(o, Transform) and self.key() == o.key()
@@ -435,7 +438,16 @@ class CudaBackend:
         out = self.dev_alloc(cap)
         ot = out_type_slot(max(q_slots_of(final), quick_q_of(base_type, transforms)), keep)
         nb = C.c_size_t()
+        sides = []  # (device buffer, host array, written by the fold)
         try:
+            # the result stays on the device, and so do the side arrays while the fold runs
+            for x, t in zip(ch, transforms):
+                for name in ("side0", "side1"):
+                    host = getattr(t, name)
+                    if t.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX) and isinstance(host, np.ndarray):
+                        sides.append((self.dev_alloc(host.nbytes), host, t.kind == A.X_QUANTIZE_MX))
+                        self.upload(sides[-1][0], host)
+                        setattr(x, name, sides[-1][0])
             self.fill_zero(out, cap)
             if isinstance(data, ResidentContent):
                 src, n, on_dev = data.buf, data.nbytes, 1
@@ -445,9 +457,15 @@ class CudaBackend:
             rc = self.lib.b200c_fold(self.ctx, C.byref(bt), src, n, int(is_splat), on_dev, ch, len(transforms), out, cap, 1,
                                      C.byref(nb), C.byref(ot), 0)
             raise_for(rc, self._err())
+            for dev, host, written in sides:
+                if written:
+                    host.view(np.uint8).reshape(-1)[:] = self.download(dev, host.nbytes)
         except Exception:
             self.dev_free(out)
             raise
+        finally:
+            for dev, _, _ in sides:
+                self.dev_free(dev)
         t = NDType.from_c(ot)
         return ResidentContent(self, t, out, max(t.getTotalAllocSize(), nb.value), nb.value)
 
@@ -830,6 +848,46 @@ class ContentAttr:
         s1 = np.zeros(oc, dtype=np.int32)
         out = self.addTransformation(Transform(A.X_QUANTIZE_SYNTH, i0=scheme, side0=s0, side1=s1))
         return out
+
+    def quantizeMx(self, fmt, tensorScale=0.0):
+        """Block-scaled 4-bit floats (A.MXFP4 or A.NVFP4; no reference counterpart): the element type becomes F4E2M1, the
+        blocks run along the innermost memory dimension, a multiple of 32.  The scales [rows, blocks] land in the
+        returned attribute's `.mxScales`, for nvfp4 the tensor scale (found from the data when 0) and the largest
+        magnitude in `.mxTensorScale`."""
+        mem = self.getType().getMemShape()
+        cols = mem[-1] if mem else 0
+        rows = int(np.prod(mem[:-1], dtype=np.int64))
+        s0 = np.zeros((rows, -(-cols // (32 if fmt == A.MXFP4 else 16))), np.uint8)
+        s1 = np.zeros(2, np.float32) if fmt == A.NVFP4 else None
+        return self.addTransformation(Transform(A.X_QUANTIZE_MX, i0=fmt, f=tensorScale, side0=s0, side1=s1))
+
+    def dequantizeMx(self, fmt, elem, scales=None, tensorScale=None):
+        """What 4-bit floats stand for, as `elem` (A.F16, A.BF16 or A.F32).  scales (uint8 [rows, blocks]) and, for nvfp4,
+        tensorScale (float32, the first counts): arrays, or None right behind a quantizeMx."""
+        s0 = None if scales is None else np.ascontiguousarray(scales, np.uint8)
+        s1 = None if tensorScale is None else np.ascontiguousarray(tensorScale, np.float32).reshape(-1)
+        if s0 is not None:
+            mem = self.getType().getMemShape()
+            want = int(np.prod(mem[:-1], dtype=np.int64)) * -(-(mem[-1] if mem else 0) // (32 if fmt == A.MXFP4 else 16))
+            if s0.size != want:
+                raise ConstError(f"DequantizeMx: {s0.size} scales for {want} blocks")
+        if s1 is not None and s1.size < 1:
+            raise ConstError("DequantizeMx: empty tensor scale")
+        return self.addTransformation(Transform(A.X_DEQUANTIZE_MX, i0=fmt, elem=elem, side0=s0, side1=s1))
+
+    def _sideOf(self, kind, name):
+        for t in reversed(self._transforms):
+            if t.kind == kind:
+                return getattr(t, name)
+        return None
+
+    @property
+    def mxScales(self):
+        return self._sideOf(A.X_QUANTIZE_MX, "side0")
+
+    @property
+    def mxTensorScale(self):
+        return self._sideOf(A.X_QUANTIZE_MX, "side1")
 
     @property
     def sideScales(self):

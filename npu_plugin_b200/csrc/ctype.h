@@ -65,7 +65,7 @@ inline bool dtValid(int dt) {
     const int b = dtBits(dt);
     switch (dtClass(dt)) {
     case B200C_CLS_FLOAT:
-        return b == 16 || b == 32 || b == 64;
+        return b == 4 || b == 16 || b == 32 || b == 64;
     case B200C_CLS_BFLOAT:
         return b == 16;
     case B200C_CLS_INT:

@@ -75,10 +75,13 @@ private:
     void* uploadTable(const void* host, size_t bytes);
     void needByteStorage(const char* what);
     void quantizeSynth(const Transformation& x, const TensorType& outType);
+    void quantizeMx(const Transformation& x, const TensorType& outType);
+    void dequantizeMx(const Transformation& x, const TensorType& outType);
+    void* finalOrScratch(size_t bytes);
     void getSparsityMap(const TensorType& outType, int swizzleKey);
     void sparsify(const Transformation& x);
     void subviewBits(const Transformation& x, const TensorType& outType);
-    void swizzle(const Transformation& x, const TensorType& outType);
+    void swizzle(const Transformation& x, const TensorType& outType, long long keepRawBytes);
     size_t emitCopyTo(void* dst, size_t cap, int swizzleKey, int64_t totalBytes);
     void runGeneric(const GenParams& p);
     void remapDense(GenParams p, int tag, const TensorType& outType, int storage);
@@ -98,6 +101,7 @@ private:
     Context* _ctx;
     ContentState _s;
     std::vector<SideOutput> _sides;
+    b200c_mx_matrix _mx = {};  // the last QuantizeMx of the chain: its scales, for a DequantizeMx behind it
     bool _afterBitPack = false;
     bool _sideOnDevice = false;
     bool _emittingFinal = false;  // the kernel being issued writes the caller's output and nothing reads it later
