@@ -3,8 +3,7 @@
 //
 // sum_k A[i][k] B[j][k] with A[i][k] = code * scale: tcgen05.mma takes the codes from shared memory and the
 // scales from tensor memory and multiplies both in, 64 elements of k at a time; sums are 32 bits wide.
-// One side's rows are the 128 rows of a tile ("P"), the other's its columns ("Q"); the wider side is P when
-// the other has few rows, since 128 is the only height there is.
+// One side's rows are the 128 rows of a tile ("P"), the other's its columns ("Q").
 #include "mx.h"
 #include "runtime.h"
 
@@ -35,8 +34,7 @@ struct MxMatmulParams {
     void* out;
     long long ld;
     int outTag;            // T_F16, T_BF16, T_F32
-    int across;            // out[q * ld + p] instead of out[p * ld + q]
-    int wide;              // 16-byte stores along a row are aligned
+    int wide;              // rows of the product are 16-byte aligned
     int* err;
 };
 
@@ -52,13 +50,14 @@ struct Tile {
     static constexpr int bytesQ = BN * 128;
     static constexpr int scaleBytes = chunksPerTile * 512;  // of each side: a tile of Q begins where 128 rows do
     static constexpr int stageBytes = (bytesP + bytesQ + 2 * scaleBytes + 1023) / 1024 * 1024;
-    static constexpr int stages = BN <= 16 ? 5 : BN <= 32 ? 4 : 3;         // two CTAs fit an SM
+    // two CTAs fit an SM; more stages where one CTA has it to itself gained nothing
+    static constexpr int stages = BN <= 16 ? 5 : BN <= 32 ? 4 : 3;
     static constexpr int smemBytes = 1024 /* alignment */ + stages * stageBytes;
     static constexpr int scaleCols = 2 * chunksPerTile * 4;  // tensor memory columns of a stage's scales
     static constexpr int scaleBufs = 2;
     static constexpr int needCols = BN + scaleBufs * scaleCols;
     static constexpr int cols = needCols <= 64 ? 64 : needCols <= 128 ? 128 : 256;
-    static_assert(stages * stageBytes >= 128 * BN * 4, "the partial sums of a split tile use the stages' memory");
+    static_assert(stages * stageBytes >= 128 * BN * 4, "the sums of a tile use the stages' memory on their way out");
 };
 
 // Two CTAs, 256 rows of P by 256 rows of Q: each CTA holds 128 rows of both sides and the sums of its 128
@@ -313,40 +312,39 @@ __device__ __forceinline__ float toOut<float>(float v) {
     return v;
 }
 
-// N accumulator columns of row p, columns q0.. of the product
+// The single-CTA kernel's P is the right matrix: N accumulator columns of lane p are N rows of the product at column p, and
+// a warp's lanes store 32 neighbours at a time.
 template <class T, int N>
-__device__ __forceinline__ void storeColumns(const MxMatmulParams& g, long long p, long long q0, const float* v) {
+__device__ __forceinline__ void storeAcross(const MxMatmulParams& g, long long p, long long q0, const float* v) {
     if (p >= g.rowsP) return;
     const long long left = g.rowsQ - q0;
-    T* out = static_cast<T*>(g.out);
-    if (g.across) {
+    T* at = static_cast<T*>(g.out) + q0 * g.ld + p;
+    if (left >= N) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < left) out[(q0 + i) * g.ld + p] = toOut<T>(v[i]);
-        return;
+        for (int i = 0; i < N; ++i, at += g.ld) *at = toOut<T>(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i, at += g.ld)
+            if (i < left) *at = toOut<T>(v[i]);
     }
-    T* row = out + p * g.ld + q0;
-    constexpr int per = N < static_cast<int>(16 / sizeof(T)) ? N : 16 / sizeof(T);
+}
+// The pair kernel's P is the left matrix.  Where its bulk stores cannot be used -- rows that are not 16-byte aligned --
+// a thread stores along its row.
+template <class T, int N>
+__device__ __forceinline__ void storeAlong(const MxMatmulParams& g, long long p, long long q0, const float* v) {
+    if (p >= g.rowsP) return;
+    const long long left = g.rowsQ - q0;
+    T* row = static_cast<T*>(g.out) + p * g.ld + q0;
 #pragma unroll
-    for (int i = 0; i < N; i += per) {
-        if (N >= static_cast<int>(16 / sizeof(T)) && g.wide && i + per <= left) {
-            alignas(16) T t[per];
-#pragma unroll
-            for (int j = 0; j < per; ++j) t[j] = toOut<T>(v[i + j]);
-            *reinterpret_cast<uint4*>(row + i) = *reinterpret_cast<const uint4*>(t);
-        } else {
-#pragma unroll
-            for (int j = 0; j < per; ++j)
-                if (i + j < left) row[i + j] = toOut<T>(v[i + j]);
-        }
-    }
+    for (int i = 0; i < N; ++i)
+        if (i < left) row[i] = toOut<T>(v[i]);
 }
 
 template <class T, int BN>
 __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int acc, long long p, long long q0, float alpha) {
     constexpr int n = BN < 32 ? BN : 32;
 #pragma unroll 1
-    for (int c = 0; c < BN; c += n) {
+    for (int c = 0; c < BN && q0 + c < g.rowsQ; c += n) {
         float v[32];
         if (n == 32) {
             readColumns(acc + c, v);
@@ -355,12 +353,12 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
         }
 #pragma unroll
         for (int i = 0; i < n; ++i) v[i] = v[i] * alpha;
-        storeColumns<T, n>(g, p, q0 + c, v);
+        storeAcross<T, n>(g, p, q0 + c, v);
     }
 }
 
-// The tile's sums lie in `split` (at most MOST) CTAs' shared memory as [BN][128]; this CTA adds up its share of the
-// columns, in the order of the ranks.  A thread takes four rows at a time, and 16 loads from the cluster's memory
+// A tile whose k is shared out: its sums lie
+// in `split` (at most MOST) CTAs' shared memory as [BN][128]; this CTA adds up its share of the columns, in the order of the ranks.  A thread takes four rows at a time, and 16 loads from the cluster's memory
 // are under way at once: with one column at a time the waiting for them took longer than the product itself.
 template <class T, int BN, int MOST>
 __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0,
@@ -402,7 +400,7 @@ __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned in
                 v[i] = toOut<T>(s * alpha);
             }
             T* out = static_cast<T*>(g.out);
-            if (g.across && g.wide && rows == 4) {
+            if (g.wide && rows == 4) {
                 T* at = out + q * g.ld + p;
                 if (sizeof(T) == 4) {
                     *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(v);
@@ -412,7 +410,7 @@ __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned in
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (i < rows) out[g.across ? q * g.ld + p + i : (p + i) * g.ld + q] = v[i];
+                    if (i < rows) out[q * g.ld + p + i] = v[i];
             }
         }
     }
@@ -440,6 +438,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     __shared__ int stalledWord;
     volatile int* stalled = &stalledWord;
     const unsigned int stage0 = (smemAddr(raw) + 1023u) & ~1023u;
+    constexpr int stages = S::stages;
     const unsigned int full = smemAddr(bars), empty = full + 8 * S::stages, done = empty + 8 * S::stages;
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const unsigned int rank = g.split > 1 ? clusterRank() : 0;
@@ -452,7 +451,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     if (threadIdx.x == 0) {
         prefetchMap(&mapP);
         prefetchMap(&mapQ);
-        for (int s = 0; s < S::stages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             barInit(full + 8 * s, 1);
             barInit(empty + 8 * s, 1);
         }
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         const long long scaleTileP = p0 / 128, scaleTileQ = q0 / 128;
         int s = 0, phase = 1, issued = 0;
         for (; issued < n; ++issued) {
-            if (!__all_sync(0xFFFFFFFFu, issued < S::stages || barWait(empty + 8 * s, phase, stalled))) break;
+            if (!__all_sync(0xFFFFFFFFu, issued < stages || barWait(empty + 8 * s, phase, stalled))) break;
             if (electOne()) {
                 const int kt = k0 + issued;
                 const unsigned int at = stage0 + s * S::stageBytes, bar = full + 8 * s;
@@ -489,51 +488,62 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
                 loadBytes(sp + S::scaleBytes, g.scalesQ + (scaleTileQ * g.chunks + chunk) * 512, scaleBytes, bar);
             }
             __syncwarp();
-            if (++s == S::stages) s = 0, phase ^= 1;
+            if (++s == stages) s = 0, phase ^= 1;
         }
         // a wait that gave up leaves copies in flight: they write this CTA's memory, so it stays until they have
         if (*stalled) {
-            for (int i = max(0, issued - S::stages); i < issued; ++i) drain(full + 8 * (i % S::stages), (i / S::stages) & 1);
+            for (int i = max(0, issued - stages); i < issued; ++i) drain(full + 8 * (i % stages), (i / stages) & 1);
         }
     } else if (warp == 5) {
         const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesP);
         const unsigned long long ds0 = scaleDesc(stage0 + S::bytesP + S::bytesQ);
-        int s = 0, phase = 0;
+        int s = 0, phase = 0, before = 0, beforePhase = 0;  // before: the stage scaleBufs ago
         for (int i = 0; i < n; ++i) {
-            bool ok = barWait(full + 8 * s, phase, stalled);
+            if (!__all_sync(0xFFFFFFFFu, barWait(full + 8 * s, phase, stalled))) break;
             // the scales' columns are free once the products that read them are done: nothing else orders a copy behind them
-            if (i >= S::scaleBufs) ok = ok && barWait(empty + 8 * ((i - S::scaleBufs) % S::stages), ((i - S::scaleBufs) / S::stages) & 1, stalled);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (i >= S::scaleBufs) {
+                if (!__all_sync(0xFFFFFFFFu, barWait(empty + 8 * before, beforePhase, stalled))) break;
+                if (++before == stages) before = 0, beforePhase ^= 1;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (electOne()) {
                 const int kt = k0 + i;
                 const unsigned int colP = scaleCol + (i % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
                 const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
-                const bool whole = kt + 1 < g.ktiles;
-                const int chunks = whole ? S::chunksPerTile : static_cast<int>(g.chunks - static_cast<long long>(kt) * S::chunksPerTile);
-                const int steps = whole ? kTileK / kStepK : static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+                if (kt + 1 < g.ktiles) {
 #pragma unroll
-                for (int c = 0; c < S::chunksPerTile; ++c) {
-                    if (c < chunks) {
+                    for (int c = 0; c < S::chunksPerTile; ++c) {
                         copyScales(colP + c * 4, ds0 + off + c * 32);
                         copyScales(colQ + c * 4, ds0 + off + S::scaleBytes / 16 + c * 32);
                     }
+                    mmaStage<128, BN, NV, false>(acc, dp0 + off, dq0 + off, colP, colQ, 4, kTileK / kStepK, i == 0);
+                } else {  // the last of k: what scales there are
+                    const int chunks = static_cast<int>(g.chunks - static_cast<long long>(kt) * S::chunksPerTile);
+                    const int steps = static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+#pragma unroll
+                    for (int c = 0; c < S::chunksPerTile; ++c) {
+                        if (c < chunks) {
+                            copyScales(colP + c * 4, ds0 + off + c * 32);
+                            copyScales(colQ + c * 4, ds0 + off + S::scaleBytes / 16 + c * 32);
+                        }
+                    }
+                    mmaStage<128, BN, NV, false>(acc, dp0 + off, dq0 + off, colP, colQ, 4, steps, i == 0);
                 }
-                mmaStage<128, BN, NV, false>(acc, dp0 + off, dq0 + off, colP, colQ, 4, steps, i == 0);
                 mmaCommit(empty + 8 * s);
                 if (i + 1 == n) mmaCommit(done);
             }
             __syncwarp();
-            if (++s == S::stages) s = 0, phase ^= 1;
+            if (++s == stages) s = 0, phase ^= 1;
         }
     }
+    __syncwarp();
     const bool finished = warp < 4 && __all_sync(0xFFFFFFFFu, barWait(done, 0, stalled) && !*stalled);  // the reads are the whole warp's
     const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
     const unsigned int mine = acc + (static_cast<unsigned int>(warp * 32) << 16);
     const int row = warp * 32 + lane;
+    if (finished) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (g.split == 1) {
         if (finished) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (g.outTag == T_F16) {
                 epilogue<__half, BN>(g, mine, p0 + row, q0, alpha);
             } else if (g.outTag == T_BF16) {
@@ -544,10 +554,9 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         }
     } else {
         if (finished) {  // all products are done with the stages
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             constexpr int w = BN < 32 ? BN : 32;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += w) {
+            for (int c = 0; c < BN && q0 + c < g.rowsQ; c += w) {
                 float v[32];
                 if (w == 32) {
                     readColumns(mine + c, v);
@@ -603,7 +612,7 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * alpha;
     if (!g.wide) {
-        storeColumns<T, 32>(g, row0 + lane, col0, v);
+        storeAlong<T, 32>(g, row0 + lane, col0, v);
         return;
     }
     constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16, bufs = 2 * 128 / rowBytes;
@@ -728,7 +737,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
         if (*stalled && rank == 0) {  // copies in flight write both CTAs' memory, which stays until they have
             for (int i = max(0, issued - S::stages); i < issued; ++i) drain(full + 8 * (i % S::stages), (i / S::stages) & 1);
         }
-    } else if (warp == 5 && rank == 0 && electOne()) {
+    } else if (warp == 5 && rank == 0) {
         const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesSide);
         const unsigned long long ds0 = scaleDesc(stage0 + 2 * S::bytesSide);
         int s = 0, phase = 0, it = 0, done = 0;
@@ -736,7 +745,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
         bool ok = true;
         for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs, ++done) {
             const unsigned int acc = tmem + (done & 1) * S::accStep;
-            if (done > 0) ok = barWait(accFree, (done - 1) & 1, stalled);
+            if (done > 0) ok = __all_sync(0xFFFFFFFFu, barWait(accFree, (done - 1) & 1, stalled));
             for (int kt = 0; kt < g.ktiles && ok; ++kt, ++it) {
                 ok = barWait(full + 8 * s, phase, stalled);
                 // as above: a copy of scales waits for the products that read the columns before
@@ -744,24 +753,28 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
                     ok = ok && barWait(empty + 8 * before, beforePhase, stalled);
                     if (++before == S::stages) before = 0, beforePhase ^= 1;
                 }
+                ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned int colP = tmem + S::scaleCol + (it % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
-                const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
+                if (electOne()) {
+                    const unsigned int colP = tmem + S::scaleCol + (it % S::scaleBufs) * S::scaleCols, colQ = colP + S::chunksPerTile * 4;
+                    const unsigned long long off = static_cast<unsigned long long>(s * (S::stageBytes >> 4));
 #pragma unroll
-                for (int c = 0; c < S::chunksPerTile; ++c) {
-                    copyScalesPair(colP + c * 4, ds0 + off + c * 32);
-                    copyScalesPair(colQ + c * 8, ds0 + off + S::scaleBytes / 16 + c * 32);
-                    copyScalesPair(colQ + c * 8 + 4, ds0 + off + S::scaleBytes / 8 + c * 32);
+                    for (int c = 0; c < S::chunksPerTile; ++c) {
+                        copyScalesPair(colP + c * 4, ds0 + off + c * 32);
+                        copyScalesPair(colQ + c * 8, ds0 + off + S::scaleBytes / 16 + c * 32);
+                        copyScalesPair(colQ + c * 8 + 4, ds0 + off + S::scaleBytes / 8 + c * 32);
+                    }
+                    if (kt + 1 < g.ktiles) {
+                        mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, kTileK / kStepK, kt == 0);
+                    } else {
+                        const int steps = static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
+                        mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, steps, kt == 0);
+                    }
+                    mmaCommitPair(empty + 8 * s);
+                    if (kt + 1 == g.ktiles) mmaCommitPair(accFull);
                 }
-                if (kt + 1 < g.ktiles) {
-                    mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, kTileK / kStepK, kt == 0);
-                } else {
-                    const int steps = static_cast<int>((g.k - static_cast<long long>(kt) * kTileK + kStepK - 1) / kStepK);
-                    mmaStage<256, 256, NV, true>(acc, dp0 + off, dq0 + off, colP, colQ, 8, steps, kt == 0);
-                }
-                mmaCommitPair(empty + 8 * s);
-                if (kt + 1 == g.ktiles) mmaCommitPair(accFull);
+                __syncwarp();
                 if (++s == S::stages) s = 0, phase ^= 1;
             }
         }
@@ -919,9 +932,12 @@ void launchTileOf(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix&
     g.tilesQ = static_cast<int>((q.rows + BN - 1) / BN);
     const long long tiles = static_cast<long long>(g.tilesP) * g.tilesQ;
     g.split = splitOf(ctx, tiles, g.ktiles, BN);
+#ifdef FORCE_SPLIT
+    if (const char* e = std::getenv("MXSPLIT")) if (std::atoi(e)) g.split = std::min(g.ktiles, std::atoi(e));
+#endif
     if (tiles * g.split > 0x7FFFFFFFll) throw BadArg("the product has too many tiles");
-    launchClusters(ctx, mxMatmulKernel<BN, NV>, static_cast<unsigned int>(tiles * g.split), static_cast<unsigned int>(g.split), S::smemBytes,
-                   mapOf(p, 128), mapOf(q, BN), g);
+    launchClusters(ctx, mxMatmulKernel<BN, NV>, static_cast<unsigned int>(tiles * g.split), static_cast<unsigned int>(g.split),
+                   S::smemBytes, mapOf(p, 128), mapOf(q, BN), g);
 }
 
 template <bool NV>
@@ -961,9 +977,8 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     }
     const long long big = ((a.rows + 255) / 256) * ((b.rows + 255) / 256);
     const bool pairs = big >= ctx->smCount / 4 && a.rows > 128 && b.rows > 128;
-    const bool across = !pairs && a.rows < b.rows;
-    const b200c_mx_matrix& p = across ? b : a;
-    const b200c_mx_matrix& q = across ? a : b;
+    const b200c_mx_matrix& p = pairs ? a : b;
+    const b200c_mx_matrix& q = pairs ? b : a;
     const bool nv = a.format == B200C_NVFP4;
     MxMatmulParams g;
     g.scalesP = static_cast<const unsigned char*>(p.scales);
@@ -981,7 +996,6 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     g.out = out;
     g.ld = outLd;
     g.outTag = dtype == B200C_F16 ? T_F16 : dtype == B200C_BF16 ? T_BF16 : T_F32;
-    g.across = across;
     g.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (outLd * es) % 16 == 0;
     g.err = ctx->errWord;
     if (pairs) {
