@@ -24,13 +24,15 @@ struct MxQuantParams {
     unsigned char* scales;
     int tiled;
     float* tensorScale;
-    int scaleGiven;
+    int scaleFrom;  // nvfp4: where t comes from
     void* values;  // or nullptr
     long long valuesLd;
     long long blocks;       // blocks of a row
     long long scaleRows;    // rows of scale bytes, those that fill up the last tile included
     long long scaleBlocks;  // the same for blocks
 };
+
+enum : int { kScaleGiven, kScaleFound /* tensorScale[1] holds the largest magnitude */, kScaleHere /* the kernel looks for it */ };
 
 struct MxDequantParams {
     const unsigned char* codes;
@@ -126,19 +128,92 @@ struct Raw {
     static constexpr int n = 8 * sizeof(T) / 16;
     uint4 v[n];
 };
-// `wide`: 16-byte loads are aligned.  Behind the last column: zeros.
-template <class T, bool WIDE>
+// 16-byte loads that are aligned: all eight are there, or none
+template <class T>
 __device__ __forceinline__ Raw<T> load8(const T* p, int left) {
     Raw<T> r;
-    if (WIDE) {  // all eight or none
 #pragma unroll
-        for (int i = 0; i < Raw<T>::n; ++i) r.v[i] = left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
-    } else {
+    for (int i = 0; i < Raw<T>::n; ++i) r.v[i] = left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+    return r;
+}
+
+// Rows that start anywhere (aligned to their elements): memory is read and written in whole 16-byte lines all the same.
+// A thread's eight elements begin m bytes into a line, m the same along a row; what it lacks of its last line is the
+// first line of the next thread, and the bytes are shifted into place.  The first and last line that a warp has of
+// a row hold bytes of others, too: they are read, never written whole -- a line that holds one byte of a matrix lies in
+// the same allocation as that byte.
+//
+// N words, `bytes` (0 .. 15) on from the start of z
+template <int N>
+__device__ __forceinline__ void shifted(const unsigned int z[N + 4], unsigned int bytes, unsigned int out[N]) {
+    unsigned int a[N + 2], b[N + 1];
+#pragma unroll
+    for (int i = 0; i < N + 2; ++i) a[i] = bytes & 8 ? z[i + 2] : z[i];
+#pragma unroll
+    for (int i = 0; i < N + 1; ++i) b[i] = bytes & 4 ? a[i + 1] : a[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(b[i], b[i + 1], (bytes & 3) * 8);
+}
+// hasNext: the next thread of the warp has the next eight elements of the row.  Whole warps call this.
+template <class T>
+__device__ __forceinline__ Raw<T> loadAny(const T* p, int left, bool hasNext) {
+    constexpr int n = Raw<T>::n;
+    const unsigned int m = static_cast<unsigned int>(reinterpret_cast<uintptr_t>(p) & 15);
+    const uint4* line = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - m);
+    const int valid = min(max(left, 0), 8) * static_cast<int>(sizeof(T));
+    unsigned int w[4 * n + 4];
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+        uint4 l = make_uint4(0, 0, 0, 0);
+        if (valid > 0 && static_cast<int>(m) + valid > 16 * k) l = __ldcs(line + k);
+        w[4 * k] = l.x, w[4 * k + 1] = l.y, w[4 * k + 2] = l.z, w[4 * k + 3] = l.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[4 * n + i] = __shfl_down_sync(0xFFFFFFFFu, w[i], 1);
+    if ((!hasNext || left <= 8) && static_cast<int>(m) + valid > 16 * n) {
+        const uint4 l = __ldcs(line + n);
+        w[4 * n] = l.x, w[4 * n + 1] = l.y, w[4 * n + 2] = l.z, w[4 * n + 3] = l.w;
+    }
+    Raw<T> r;
+    shifted<4 * n>(w, m, reinterpret_cast<unsigned int*>(r.v));
+    if (left < 8) {
         T* t = reinterpret_cast<T*>(r.v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = i < left ? p[i] : fromFloat<T>(0.f);
+        for (int i = 0; i < 8; ++i)
+            if (i >= left) t[i] = fromFloat<T>(0.f);
     }
     return r;
+}
+template <class T>
+__device__ __forceinline__ void storeAny(T* p, int left, const T t[8], bool hasPrev, bool hasNext) {
+    constexpr int n = Raw<T>::n, es = sizeof(T);
+    const int m = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    const int valid = min(max(left, 0), 8) * es;
+    const unsigned int* v = reinterpret_cast<const unsigned int*>(t);
+    unsigned int z[4 * n + 4], o[4 * n];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = __shfl_up_sync(0xFFFFFFFFu, v[4 * n - 4 + i], 1);
+#pragma unroll
+    for (int i = 0; i < 4 * n; ++i) z[4 + i] = v[i];
+    shifted<4 * n>(z, (16 - m) & 15, o);
+    uint4* line = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - m);
+    // the bytes of this thread's that lines take: from the start, or the second line if the first one has others' bytes
+    int from = m == 0 || hasPrev ? 0 : 16 - m, to = from;
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+        if (valid >= 16 * (k + 1) - m && (k > 0 || from == 0)) {
+            __stcs(line + k, m == 0 ? make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3])
+                                    : make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+            to = 16 * (k + 1) - m;
+        }
+    }
+    // the next thread's first line takes the last m bytes, if it is written whole
+    const int end = hasNext && (left - 8) * es >= 16 - m ? min(valid, 16 * n - m) : valid;
+    if (from > 0 || to < end) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((i * es < from || i * es >= to) && i * es < end) p[i] = t[i];
+    }
 }
 template <class T>
 __device__ __forceinline__ void unpack8(const Raw<T>& r, float v[8]) {
@@ -146,12 +221,11 @@ __device__ __forceinline__ void unpack8(const Raw<T>& r, float v[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = toFloat<T>(t[i]);
 }
-// what eight codes with the factor d stand for -> p.  `power`: d is a power of two
-template <class T, bool WIDE, bool POWER>
-__device__ __forceinline__ void storeValues(T* p, int left, unsigned int word, float d) {
+// what eight codes with the factor d stand for; `POWER`: d is a power of two
+template <class T, bool POWER>
+__device__ __forceinline__ void values8(unsigned int word, float d, T t[8]) {
     __half2 h[4];
     valuesOf(word, h);
-    alignas(16) T t[8];
     if (sizeof(T) == 2 && POWER && std::is_same<T, __half>::value && d >= 5.9604645e-8f && d <= 32768.f) {
         // a factor that f16 has: the product is rounded once, and only where it is subnormal or too large
         const __half2 f = __half2half2(__float2half_rn(d));
@@ -165,14 +239,11 @@ __device__ __forceinline__ void storeValues(T* p, int left, unsigned int word, f
             t[2 * i + 1] = fromFloat<T>(c.y * d);
         }
     }
-    if (WIDE) {
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, const T t[8]) {
 #pragma unroll
-        for (int i = 0; i < Raw<T>::n; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(t)[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = t[i];
-    }
+    for (int i = 0; i < Raw<T>::n; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(t)[i]);
 }
 // largest magnitude of the eight, as the bits of a 32-bit float: bits of magnitudes order like the magnitudes,
 // for 16-bit types two at a time
@@ -229,37 +300,80 @@ struct Lay {
 
 // largest finite magnitude of the matrix -> tensorScale[1] (zeroed before).  A maximum does not depend on the
 // order it is taken in.
+// the largest finite magnitude among eight elements and `top`
+template <class T>
+__device__ __forceinline__ unsigned int topFinite(unsigned int top, const Raw<T>& raw) {
+    const unsigned int m = top8<T>(raw);
+    if (m < 0x7F800000u) return max(top, m);
+    float v[8];  // a NaN or an infinity hides the others
+    unpack8<T>(raw, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const unsigned int a = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        if (a < 0x7F800000u) top = max(top, a);
+    }
+    return top;
+}
+
+// the row of the first thread of this thread's warp within its CTA
+__device__ __forceinline__ int warpRow(int x) {
+    const int thread = threadIdx.y * blockDim.x + threadIdx.x;
+    return (thread & ~31) / x;
+}
+
 template <class T, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQuantParams p) {
     typedef Lay<UNITS> L;
     afterLast();
+    const int x = L::x(), lane = (threadIdx.y * x + threadIdx.x) & 31;
+    const bool hasNext = (lane & (min(x, 32) - 1)) != min(x, 32) - 1;
+    const int cols = static_cast<int>(p.cols), units = (cols + 7) / 8;
     unsigned int top = 0;
-    const int units = static_cast<int>((p.cols + 7) / 8), cols = static_cast<int>(p.cols);
-    for (long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; r < p.rows; r += static_cast<long long>(gridDim.x) * blockDim.y) {
-        for (int u = L::firstUnit(); u < units; u += L::unitStep()) {
-            const T* src = static_cast<const T*>(p.src) + r * p.srcLd + u * 8ll;
+    // rows of the warp's first thread
+    for (long long r0 = static_cast<long long>(blockIdx.x) * blockDim.y + warpRow(x); r0 < p.rows; r0 += static_cast<long long>(gridDim.x) * blockDim.y) {
+        for (int base = L::firstUnit() - static_cast<int>(threadIdx.x); base < units; base += L::unitStep()) {
+            const int u = base + threadIdx.x;
             Raw<T> raw[UNITS];
 #pragma unroll
-            for (int i = 0; i < UNITS; ++i) raw[i] = load8<T, WIDE>(src + i * L::x() * 8, cols - 8 * (u + i * L::x()));
-#pragma unroll
             for (int i = 0; i < UNITS; ++i) {
-                const unsigned int m = top8<T>(raw[i]);
-                if (m < 0x7F800000u) {
-                    top = max(top, m);
-                } else {  // a NaN or an infinity hides the others
-                    float v[8];
-                    unpack8<T>(raw[i], v);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const unsigned int a = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-                        if (a < 0x7F800000u) top = max(top, a);
-                    }
+                if (WIDE) {
+                    const long long r = r0 + (x < 32 ? lane / x : 0);
+                    raw[i] = load8<T>(static_cast<const T*>(p.src) + r * p.srcLd + (u + i * x) * 8ll, r < p.rows ? cols - 8 * (u + i * x) : 0);
+                } else {
+                    const long long r = r0 + (x < 32 ? lane / x : 0);
+                    raw[i] = loadAny<T>(static_cast<const T*>(p.src) + r * p.srcLd + (u + i * x) * 8ll, r < p.rows ? cols - 8 * (u + i * x) : 0, hasNext);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) top = topFinite<T>(top, raw[i]);
         }
     }
     top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if (((threadIdx.y * blockDim.x + threadIdx.x) & 31) == 0 && top) atomicMax(reinterpret_cast<unsigned int*>(p.tensorScale) + 1, top);
+    if (lane == 0 && top) atomicMax(reinterpret_cast<unsigned int*>(p.tensorScale) + 1, top);
+}
+
+// The same by one CTA alone, for a small matrix: this thread's warp's share.
+template <class T, bool WIDE>
+__device__ __forceinline__ unsigned int topHere(const MxQuantParams& p, int thread, int threads) {
+    constexpr int batch = WIDE ? 4 : 2, each = WIDE ? 8 : 1;  // of 8 elements under way at once; neighbours of one load
+    const int cols = static_cast<int>(p.cols), across = (cols + each - 1) / each, n = static_cast<int>(p.rows) * across;
+    unsigned int top = 0;
+    for (int first = thread; first < n; first += threads * batch * 8 / each) {
+        Raw<T> raw[batch];
+#pragma unroll
+        for (int i = 0; i < batch * 8 / each; ++i) {
+            const int at = first + i * threads, r = at / across, c = at - r * across;
+            const T* from = static_cast<const T*>(p.src) + r * p.srcLd + c * each;
+            if (WIDE) {
+                raw[i] = load8<T>(from, at < n ? 8 : 0);
+            } else {
+                reinterpret_cast<T*>(raw)[i] = at < n ? *from : fromFloat<T>(0.f);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < batch; ++i) top = topFinite<T>(top, raw[i]);
+    }
+    return __reduce_max_sync(0xFFFFFFFFu, top);
 }
 
 // v / d in 32 bits without the divide instruction's calls: the product with 1 / d, corrected once by its
@@ -340,34 +454,52 @@ __device__ __forceinline__ unsigned int encode8(const Raw<T>& raw, unsigned int 
 template <class T, bool NV, bool WIDE, bool VALUES, int UNITS>
 __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ MxQuantParams p, int rowCtas) {
     typedef Lay<UNITS> L;
+    __shared__ unsigned int tops[8];
     afterLast();
-    float t = 1.f;
-    if (NV) {
-        if (p.scaleGiven) {
-            t = p.tensorScale[0];
-        } else {
-            t = tensorScaleOf(p.tensorScale[1]);
-            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && threadIdx.y == 0) p.tensorScale[0] = t;
-        }
-    }
-    const Divisor sixT(NV ? 6.f * t : 1.f, 0.f);
-    const bool badT = NV && !(t > 0.f && t <= 3.402823466e38f);
-    constexpr int lanes = NV ? 2 : 4;  // threads of a block
+    const int x = L::x(), thread = threadIdx.y * x + threadIdx.x, lane = thread & 31, warp = thread >> 5;
     if (static_cast<int>(blockIdx.x) >= rowCtas) {
         const int threads = blockDim.x * blockDim.y;
         const long long chunks = p.scaleBlocks / 4, n = (p.scaleRows - p.rows) * chunks;
         const long long cta = static_cast<long long>(blockIdx.x - rowCtas) * gridDim.y + blockIdx.y;
         const long long all = static_cast<long long>(gridDim.x - rowCtas) * gridDim.y * threads;
-        for (long long i = cta * threads + threadIdx.y * blockDim.x + threadIdx.x; i < n; i += all) {
+        for (long long i = cta * threads + thread; i < n; i += all) {
             *reinterpret_cast<unsigned int*>(p.scales + scaleAt(1, p.rows + i / chunks, i % chunks * 4, p.blocks)) = 0u;
         }
         return;
     }
+    float t = 1.f;
+    if (NV) {
+        if (p.scaleFrom == kScaleGiven) {
+            t = p.tensorScale[0];
+        } else {
+            float top;
+            if (p.scaleFrom == kScaleHere) {
+                const unsigned int mine = topHere<T, WIDE>(p, thread, blockDim.x * blockDim.y);
+                if (lane == 0) tops[warp] = mine;
+                __syncthreads();
+                unsigned int all = 0;
+                for (int i = 0; i < static_cast<int>(blockDim.x * blockDim.y) / 32; ++i) all = max(all, tops[i]);
+                top = __uint_as_float(all);
+            } else {
+                top = p.tensorScale[1];
+            }
+            t = tensorScaleOf(top);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && thread == 0) {
+                p.tensorScale[0] = t;
+                if (p.scaleFrom == kScaleHere) p.tensorScale[1] = top;
+            }
+        }
+    }
+    const Divisor sixT(NV ? 6.f * t : 1.f, 0.f);
+    const bool badT = NV && !(t > 0.f && t <= 3.402823466e38f);
+    constexpr int lanes = NV ? 2 : 4;  // threads of a block
     const int cols = static_cast<int>(p.cols), units = (cols + 31) / 32 * 4;
     const int all = max(units, static_cast<int>(p.scaleBlocks) * lanes);  // those of a tile's filling scales too
     // from the last row to the first: where the largest magnitude was looked for just before, the last rows are
     // what L2 still holds
     const long long r = p.rows - 1 - (static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y);
+    const int run = min(x, 32);  // threads of a warp that lie in one row
+    const bool hasPrev = (lane & (run - 1)) != 0, hasNext = (lane & (run - 1)) != run - 1;
     const T* src = static_cast<const T*>(p.src) + r * p.srcLd;
     unsigned char* codes = p.codes + r * p.ld;
     T* values = static_cast<T*>(p.values) + r * p.valuesLd;
@@ -378,10 +510,14 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
         const int u = base + threadIdx.x;
         Raw<T> raw[UNITS];
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) raw[i] = load8<T, WIDE>(src + u * 8ll + i * L::x() * 8, r >= 0 ? cols - 8 * (u + i * L::x()) : 0);
+        for (int i = 0; i < UNITS; ++i) {
+            const T* from = src + u * 8ll + i * x * 8;
+            const int left = r >= 0 ? cols - 8 * (u + i * x) : 0;
+            raw[i] = WIDE ? load8<T>(from, left) : loadAny<T>(from, left, hasNext);
+        }
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
-            const int ui = u + i * L::x(), left = cols - 8 * ui;
+            const int ui = u + i * x, left = cols - 8 * ui;
             unsigned int top = top8<T>(raw[i]);
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             if (!NV) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -394,7 +530,15 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
                     scales[p.tiled ? (b >> 2) * 512ll + (b & 3) : b] = static_cast<unsigned char>(left > 0 ? scale : 0u);
                 }
                 if (ui < units) *reinterpret_cast<unsigned int*>(codes + ui * 4ll) = word;
-                if (VALUES && left > 0) storeValues<T, WIDE, !NV>(values + ui * 8ll, left, word, d);
+            }
+            if (VALUES) {
+                alignas(16) T w[8];
+                values8<T, !NV>(word, d, w);
+                if (WIDE) {
+                    if (r >= 0 && left > 0) store8<T>(values + ui * 8ll, w);
+                } else {
+                    storeAny<T>(values + ui * 8ll, r >= 0 ? left : 0, w, hasPrev, hasNext);
+                }
             }
         }
     }
@@ -404,19 +548,24 @@ template <class T, bool NV, bool WIDE, int UNITS>
 __global__ void __launch_bounds__(256) mxDequantKernel(const __grid_constant__ MxDequantParams p) {
     typedef Lay<UNITS> L;
     afterLast();
+    const int x = L::x(), lane = (threadIdx.y * x + threadIdx.x) & 31;
+    const int run = min(x, 32);
+    const bool hasPrev = (lane & (run - 1)) != 0, hasNext = (lane & (run - 1)) != run - 1;
     const float t = NV ? p.tensorScale[0] : 1.f;
     const int cols = static_cast<int>(p.cols), units = (cols + 7) / 8;
     const long long r = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    if (r >= p.rows) return;
+    const bool row = r < p.rows;
     const unsigned char* codes = p.codes + r * p.ld;
-    const unsigned char* scales = p.scales + scaleAt(p.tiled, r, 0, p.blocks);
+    const unsigned char* scales = p.scales + (row ? scaleAt(p.tiled, r, 0, p.blocks) : 0);
     T* out = static_cast<T*>(p.out) + r * p.outLd;
-    for (int u = L::firstUnit(); u < units; u += L::unitStep()) {
+    for (int base = L::firstUnit() - static_cast<int>(threadIdx.x); base < units; base += L::unitStep()) {
+        const int u = base + threadIdx.x;
         unsigned int word[UNITS], scale[UNITS];
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
-            const int ui = u + i * L::x();
-            if (ui < units) {
+            const int ui = u + i * x;
+            word[i] = scale[i] = 0;
+            if (row && ui < units) {
                 const int b = ui / (NV ? 2 : 4);
                 word[i] = __ldcs(reinterpret_cast<const unsigned int*>(codes + ui * 4ll));
                 scale[i] = scales[p.tiled ? (b >> 2) * 512ll + (b & 3) : b];
@@ -424,10 +573,14 @@ __global__ void __launch_bounds__(256) mxDequantKernel(const __grid_constant__ M
         }
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
-            const int ui = u + i * L::x();
-            if (ui < units) {
-                const float d = NV ? __fmul_rn(fromE4m3(scale[i]), t) : fromE8m0(scale[i]);
-                storeValues<T, WIDE, !NV>(out + ui * 8ll, cols - 8 * ui, word[i], d);
+            const int ui = u + i * x;
+            const float d = NV ? __fmul_rn(fromE4m3(scale[i]), t) : fromE8m0(scale[i]);
+            alignas(16) T w[8];
+            values8<T, !NV>(word[i], d, w);
+            if (WIDE) {
+                if (row && ui < units) store8<T>(out + ui * 8ll, w);
+            } else {
+                storeAny<T>(out + ui * 8ll, row ? cols - 8 * ui : 0, w, hasPrev, hasNext);
             }
         }
     }
@@ -499,13 +652,13 @@ void launchTop(Context* ctx, const MxQuantParams& p) {
 
 template <class T, bool WIDE, int UNITS>
 void quantizeWith(Context* ctx, const MxQuantParams& p, bool nv) {
-    if (nv && !p.scaleGiven) {
+    if (nv && p.scaleFrom == kScaleFound) {
         fillBytes(ctx, p.tensorScale, 0, 8);
         if (p.rows > 0 && p.cols > 0) launchTop<T, WIDE, UNITS>(ctx, p);
     }
     // an empty matrix has no scales, but its factor is still written
     const long long units = std::max((p.cols + 31) / 32 * 4, p.scaleBlocks * (nv ? 2 : 4));
-    if ((p.rows == 0 || units == 0) && !(nv && !p.scaleGiven)) return;
+    if ((p.rows == 0 || units == 0) && !(nv && p.scaleFrom != kScaleGiven)) return;
     if (nv) {
         launchQuant<T, true, WIDE, UNITS>(ctx, p, units);
     } else {
@@ -563,7 +716,9 @@ void launchMxQuantize(Context* ctx, const void* src, int dtype, int64_t srcLd, c
     p.scales = static_cast<unsigned char*>(out.scales);
     p.tiled = out.scale_layout == B200C_MX_SCALES_TILED;
     p.tensorScale = out.tensor_scale;
-    p.scaleGiven = scaleGiven;
+    // up to 64 KB every CTA looks the matrix through by itself: 16 loads of a thread, where two launches before this
+    // one take about 5 us
+    p.scaleFrom = scaleGiven ? kScaleGiven : out.rows * ((out.cols + 7) / 8 * 8) * (dtBits(dtype) / 8) <= 65536 ? kScaleHere : kScaleFound;
     p.values = values;
     p.valuesLd = valuesLd;
     p.blocks = mxBlocks(out.format, out.cols);

@@ -328,18 +328,6 @@ __device__ __forceinline__ void storeAcross(const MxMatmulParams& g, long long p
             if (i < left) *at = toOut<T>(v[i]);
     }
 }
-// The pair kernel's P is the left matrix.  Where its bulk stores cannot be used -- rows that are not 16-byte aligned --
-// a thread stores along its row.
-template <class T, int N>
-__device__ __forceinline__ void storeAlong(const MxMatmulParams& g, long long p, long long q0, const float* v) {
-    if (p >= g.rowsP) return;
-    const long long left = g.rowsQ - q0;
-    T* row = static_cast<T*>(g.out) + p * g.ld + q0;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i < left) row[i] = toOut<T>(v[i]);
-}
-
 template <class T, int BN>
 __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int acc, long long p, long long q0, float alpha) {
     constexpr int n = BN < 32 ? BN : 32;
@@ -611,10 +599,6 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
     float v[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * alpha;
-    if (!g.wide) {
-        storeAlong<T, 32>(g, row0 + lane, col0, v);
-        return;
-    }
     constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16, bufs = 2 * 128 / rowBytes;
     const unsigned int at = staging + (group % bufs) * 32 * rowBytes;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(bufs - 1) : "memory");  // the last store from here has been read
@@ -628,6 +612,31 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
         // the map's swizzle: 16-byte chunks of a row of 64 or 128 bytes change places with the row's number
         const unsigned int to = at + lane * rowBytes + ((c ^ (chunks == 8 ? lane & 7 : (lane >> 1) & 3)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    }
+    if (!g.wide) {
+        // rows that no bulk store can start at: the warp stores them one by one, 32 neighbours at a time
+        __syncwarp();
+        const int rows = static_cast<int>(min(32ll, g.rowsP - row0));
+        T* out = static_cast<T*>(g.out) + row0 * g.ld + col0 + lane;
+        const bool mine = col0 + lane < g.rowsQ;
+        const int c = lane * static_cast<int>(sizeof(T)) / 16, in = lane * static_cast<int>(sizeof(T)) % 16;
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i, out += g.ld) {
+            if (i < rows && mine) {
+                const unsigned int from = at + i * rowBytes + ((c ^ (chunks == 8 ? i & 7 : (i >> 1) & 3)) << 4) + in;
+                if (sizeof(T) == 2) {
+                    unsigned short w;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+                    *reinterpret_cast<unsigned short*>(out) = w;
+                } else {
+                    unsigned int w;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+                    *reinterpret_cast<unsigned int*>(out) = w;
+                }
+            }
+        }
+        __syncwarp();
+        return;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();

@@ -18,14 +18,12 @@ def e2m1(q):
 
 def e4m3(v):
     """Non-negative 64-bit values up to 448 -> bytes, to nearest even."""
-    table = e4m3_values()[:127]
-    out = np.empty(v.shape, np.uint8)
-    flat, o = v.reshape(-1), out.reshape(-1)
-    for i, x in enumerate(flat):
-        far = np.abs(table - x)
-        near = np.flatnonzero(far == far.min())
-        o[i] = near[near % 2 == 0][0] if len(near) > 1 else near[0]
-    return out
+    table = e4m3_values()[:127]  # ascending
+    low = np.clip(np.searchsorted(table, v, side="right") - 1, 0, 126)
+    high = np.minimum(low + 1, 126)
+    down, up = v - table[low], table[high] - v
+    pick = np.where(down < up, low, np.where(up < down, high, np.where(low % 2 == 0, low, high)))
+    return pick.astype(np.uint8)
 
 
 def e4m3_values():
@@ -115,7 +113,6 @@ def lay(scales, layout):
     rows, blocks = scales.shape
     chunks = -(-blocks // 4)
     out = np.zeros(-(-rows // 128) * chunks * 512, np.uint8)
-    for r in range(rows):
-        for b in range(blocks):
-            out[((r // 128) * chunks + b // 4) * 512 + (r % 32) * 16 + (r % 128) // 32 * 4 + b % 4] = scales[r, b]
+    r, b = np.arange(rows)[:, None], np.arange(blocks)[None]
+    out[((r // 128) * chunks + b // 4) * 512 + (r % 32) * 16 + (r % 128) // 32 * 4 + b % 4] = scales
     return out

@@ -183,6 +183,26 @@ def test_quantize(dev, fmt, dtype, rows, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,dtype,cols", [(A.NVFP4, A.BF16, 4099), (A.MXFP4, A.F32, 4096), (A.NVFP4, A.F16, 4128), (A.MXFP4, A.F16, 3999)])
+def test_large_matrices(dev, fmt, dtype, cols):
+    """Enough rows for the kernels' form with several pieces of a row per thread, aligned and not, and back."""
+    rows = 1300
+    x = awkward(rows, cols, dtype, cols)
+    q = O.quantize(x.double().numpy(), fmt)
+    want = torch.from_numpy(q["values"].astype(np.float32)).to(x.dtype).nan_to_num(nan=12345.0)
+    for pad in (0, 5):
+        src = put(x, pad)
+        h = Held(fmt, rows, cols, A.MX_SCALES_TILED)
+        values = torch.full((rows, cols + pad), 7.0, dtype=x.dtype, device="cuda")
+        dev.mx_quantize(src.data_ptr(), dtype, src.stride(0), h.m, values=values.data_ptr(), values_ld=values.stride(0))
+        h.check(q)
+        assert torch.equal(values[:, :cols].cpu().nan_to_num(nan=12345.0), want) and (values[:, cols:] == 7.0).all()
+        back = torch.full((rows, cols + pad), 7.0, dtype=x.dtype, device="cuda")
+        dev.mx_dequantize(h.m, back.data_ptr(), dtype, back.stride(0))
+        assert torch.equal(back[:, :cols].cpu().nan_to_num(nan=12345.0), want) and (back[:, cols:] == 7.0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", [1.0, 0.37, 2.0 ** -9, 3e-30, 1e30])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_quantize_with_a_given_tensor_scale(dev, dtype, t):
