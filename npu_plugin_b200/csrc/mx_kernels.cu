@@ -272,8 +272,6 @@ __device__ __forceinline__ float tensorScaleOf(float top) {
     return __uint_as_float(static_cast<unsigned int>(max(e, 1)) << 23);
 }
 
-constexpr int kUnits = 4;  // units of a thread where rows are long
-
 // See mx_matmul.cu: no kernel here touches memory before the one that was launched before it has ended.
 __device__ __forceinline__ void afterLast() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -281,14 +279,13 @@ __device__ __forceinline__ void afterLast() {
 }
 
 // How a kernel's threads lie over rows x units (8 elements): x along a row, y over rows, each thread with UNITS
-// units of one row, x apart, whose loads are all under way before the first is used.  Addresses differ by
-// constants between a thread's units: with its units in different rows instead, 64-bit address arithmetic was a
-// quarter of all instructions.
-template <int UNITS>
+// units of one row, x apart, whose loads are all under way before the first is used.  X: x where it is known, 0:
+// blockDim.x.  With X = 128 the addresses of a thread's units differ by constants: with its units in different
+// rows instead, 64-bit address arithmetic was a quarter of all instructions.
+template <int UNITS, int X>
 struct Lay {
-    static constexpr int wide = 128;  // x of a thread with several units
     __device__ __forceinline__ static int x() {
-        return UNITS > 1 ? wide : static_cast<int>(blockDim.x);
+        return X ? X : static_cast<int>(blockDim.x);
     }
     __device__ __forceinline__ static int firstUnit() {
         return static_cast<int>(blockIdx.y) * x() * UNITS + static_cast<int>(threadIdx.x);
@@ -298,8 +295,6 @@ struct Lay {
     }
 };
 
-// largest finite magnitude of the matrix -> tensorScale[1] (zeroed before).  A maximum does not depend on the
-// order it is taken in.
 // the largest finite magnitude among eight elements and `top`
 template <class T>
 __device__ __forceinline__ unsigned int topFinite(unsigned int top, const Raw<T>& raw) {
@@ -321,35 +316,68 @@ __device__ __forceinline__ int warpRow(int x) {
     return (thread & ~31) / x;
 }
 
-template <class T, bool WIDE, int UNITS>
-__global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQuantParams p) {
-    typedef Lay<UNITS> L;
-    afterLast();
-    const int x = L::x(), lane = (threadIdx.y * x + threadIdx.x) & 31;
+// the largest finite magnitude of this CTA's share: a warp's first thread has its result
+template <class T, bool WIDE, int UNITS, int X>
+__device__ __forceinline__ unsigned int topOf(const MxQuantParams& p, int lane) {
+    typedef Lay<UNITS, X> L;
+    constexpr int rows = UNITS > 1 ? 1 : 4;  // of a thread, whose loads are under way together
+    const int x = L::x();
     const bool hasNext = (lane & (min(x, 32) - 1)) != min(x, 32) - 1;
     const int cols = static_cast<int>(p.cols), units = (cols + 7) / 8;
+    const long long step = static_cast<long long>(gridDim.x) * blockDim.y;
     unsigned int top = 0;
     // rows of the warp's first thread
-    for (long long r0 = static_cast<long long>(blockIdx.x) * blockDim.y + warpRow(x); r0 < p.rows; r0 += static_cast<long long>(gridDim.x) * blockDim.y) {
+    for (long long r0 = static_cast<long long>(blockIdx.x) * blockDim.y + warpRow(x); r0 < p.rows; r0 += rows * step) {
         for (int base = L::firstUnit() - static_cast<int>(threadIdx.x); base < units; base += L::unitStep()) {
             const int u = base + threadIdx.x;
-            Raw<T> raw[UNITS];
+            Raw<T> raw[UNITS * rows];
 #pragma unroll
-            for (int i = 0; i < UNITS; ++i) {
-                if (WIDE) {
-                    const long long r = r0 + (x < 32 ? lane / x : 0);
-                    raw[i] = load8<T>(static_cast<const T*>(p.src) + r * p.srcLd + (u + i * x) * 8ll, r < p.rows ? cols - 8 * (u + i * x) : 0);
-                } else {
-                    const long long r = r0 + (x < 32 ? lane / x : 0);
-                    raw[i] = loadAny<T>(static_cast<const T*>(p.src) + r * p.srcLd + (u + i * x) * 8ll, r < p.rows ? cols - 8 * (u + i * x) : 0, hasNext);
-                }
+            for (int i = 0; i < UNITS * rows; ++i) {
+                const int ui = u + (UNITS > 1 ? i * x : 0);
+                const long long r = r0 + (UNITS > 1 ? 0 : i * step) + (x < 32 ? lane / x : 0);
+                const T* from = static_cast<const T*>(p.src) + r * p.srcLd + ui * 8ll;
+                const int left = r < p.rows ? cols - 8 * ui : 0;
+                raw[i] = WIDE ? load8<T>(from, left) : loadAny<T>(from, left, hasNext);
             }
 #pragma unroll
-            for (int i = 0; i < UNITS; ++i) top = topFinite<T>(top, raw[i]);
+            for (int i = 0; i < UNITS * rows; ++i) top = topFinite<T>(top, raw[i]);
         }
     }
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    return __reduce_max_sync(0xFFFFFFFFu, top);
+}
+
+// -> tensorScale[1], zeroed before.  A maximum does not depend on the order it is taken in.
+template <class T, bool WIDE, int UNITS, int X>
+__global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQuantParams p) {
+    afterLast();
+    const int lane = (threadIdx.y * Lay<UNITS, X>::x() + threadIdx.x) & 31;
+    const unsigned int top = topOf<T, WIDE, UNITS, X>(p, lane);
     if (lane == 0 && top) atomicMax(reinterpret_cast<unsigned int*>(p.tensorScale) + 1, top);
+}
+
+// One cluster of CTAs: its first one collects the others' results, and nothing has to be zeroed before.
+template <class T, bool WIDE, int UNITS, int X>
+__global__ void __launch_bounds__(256) mxTopClusterKernel(const __grid_constant__ MxQuantParams p) {
+    __shared__ unsigned int tops[8];
+    afterLast();
+    const int thread = threadIdx.y * Lay<UNITS, X>::x() + threadIdx.x, lane = thread & 31, warps = blockDim.x * blockDim.y / 32;
+    const unsigned int top = topOf<T, WIDE, UNITS, X>(p, lane);
+    if (lane == 0) tops[thread >> 5] = top;
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (blockIdx.x == 0 && thread < 32) {
+        unsigned int all = 0;
+        for (int i = lane; i < warps * static_cast<int>(gridDim.x); i += 32) {
+            unsigned int at, v;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<unsigned int>(__cvta_generic_to_shared(tops + i % warps))), "r"(i / warps));
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+            all = max(all, v);
+        }
+        all = __reduce_max_sync(0xFFFFFFFFu, all);
+        if (lane == 0) p.tensorScale[1] = __uint_as_float(all);
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // The same by one CTA alone, for a small matrix: this thread's warp's share.
@@ -451,9 +479,9 @@ __device__ __forceinline__ unsigned int encode8(const Raw<T>& raw, unsigned int 
 
 // Whole warps go through the loop together, whatever their rows.  The last CTAs of the grid (blockIdx.x >=
 // rowCtas) zero the scales of the rows that only fill a tile up.
-template <class T, bool NV, bool WIDE, bool VALUES, int UNITS>
+template <class T, bool NV, bool WIDE, bool VALUES, int UNITS, int X>
 __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ MxQuantParams p, int rowCtas) {
-    typedef Lay<UNITS> L;
+    typedef Lay<UNITS, X> L;
     __shared__ unsigned int tops[8];
     afterLast();
     const int x = L::x(), thread = threadIdx.y * x + threadIdx.x, lane = thread & 31, warp = thread >> 5;
@@ -544,9 +572,9 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
     }
 }
 
-template <class T, bool NV, bool WIDE, int UNITS>
+template <class T, bool NV, bool WIDE, int UNITS, int X>
 __global__ void __launch_bounds__(256) mxDequantKernel(const __grid_constant__ MxDequantParams p) {
-    typedef Lay<UNITS> L;
+    typedef Lay<UNITS, X> L;
     afterLast();
     const int x = L::x(), lane = (threadIdx.y * x + threadIdx.x) & 31;
     const int run = min(x, 32);
@@ -586,31 +614,62 @@ __global__ void __launch_bounds__(256) mxDequantKernel(const __grid_constant__ M
     }
 }
 
-// rows x units of 8 elements over CTAs of up to 256 threads
-void gridFor(long long rows, long long units, int unitsOfThread, dim3* grid, dim3* block) {
-    unsigned int x = 4;
-    if (unitsOfThread > 1) {
-        x = Lay<kUnits>::wide;
-    } else {
-        while (x < 256 && x < units) x *= 2;
-    }
-    *block = dim3(x, unitsOfThread > 1 ? 1 : 256 / x);
-    const long long along = static_cast<long long>(x) * unitsOfThread;
+// rows x units of 8 elements over CTAs
+void gridFor(long long rows, int x, int threads, long long along, long long units, dim3* grid, dim3* block) {
+    *block = dim3(x, threads / x);
     *grid = dim3(static_cast<unsigned int>(std::max<long long>(1, (rows + block->y - 1) / block->y)),
                  static_cast<unsigned int>(std::max<long long>(1, std::min<long long>((units + along - 1) / along, 65535))));
 }
 
+// Which form of a kernel: threads with four units of a row where there are enough threads to fill the SMs (four CTAs
+// each) all the same, 128 along a row or -- shorter rows, or rows that would leave many of 128 idle -- fewer.
+struct Form {
+    int units, x;
+    bool fixed;  // X = 128
+};
+Form formFor(Context* ctx, long long rows, long long units) {
+    Form f{1, 4, false};
+    if (units > 8 && rows * units >= 256ll * 4 * 4 * ctx->smCount) {
+        f.units = 4;
+        long long idle = -1;
+        for (int x = 128; x >= 4; x /= 2) {
+            const long long along = 4ll * x, padded = (units + along - 1) / along * along;
+            if (idle < 0 || padded * 8 < idle * 7) {  // an eighth fewer is worth the shorter stretch
+                idle = padded;
+                f.x = x;
+            }
+        }
+        f.fixed = f.x == 128;
+    } else {
+        while (f.x < 256 && f.x < units) f.x *= 2;
+    }
+    return f;
+}
+template <class F>
+void withForm(const Form& f, F&& run) {
+    if (f.fixed) {
+        run(std::integral_constant<int, 4>(), std::integral_constant<int, 128>());
+    } else if (f.units == 4) {
+        run(std::integral_constant<int, 4>(), std::integral_constant<int, 0>());
+    } else {
+        run(std::integral_constant<int, 1>(), std::integral_constant<int, 0>());
+    }
+}
+
 template <class Kernel, class... Args>
-void launchNext(Context* ctx, Kernel kernel, dim3 grid, dim3 block, const Args&... args) {
+void launchNext(Context* ctx, Kernel kernel, dim3 grid, dim3 block, int cluster, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     ++ctx->launches;
 }
@@ -619,86 +678,78 @@ bool aligned16(const void* p, long long ldBytes) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ldBytes % 16 == 0;
 }
 
-// Several units a thread: where they leave few of its last ones idle, and enough threads to fill the SMs
-bool longRows(Context* ctx, long long rows, long long units) {
-    constexpr long long along = Lay<kUnits>::wide * kUnits;
-    const long long padded = (units + along - 1) / along * along;
-    return padded * 7 <= units * 8 && rows * units >= 256ll * kUnits * 4 * ctx->smCount;
+template <class T, bool WIDE>
+void findTop(Context* ctx, const MxQuantParams& p) {
+    const long long units = (p.cols + 7) / 8;
+    const Form f = formFor(ctx, p.rows, units);
+    dim3 grid, block;
+    gridFor(p.rows, f.x, f.fixed ? 128 : 256, static_cast<long long>(f.x) * f.units, units, &grid, &block);
+    // eight CTAs read about 1 MB in the time that zeroing the word and a grid's atomics take
+    const bool cluster = p.rows * units * 8 * static_cast<long long>(sizeof(T)) <= (1ll << 20);
+    if (!cluster) fillBytes(ctx, p.tensorScale, 0, 8);
+    grid.x = cluster ? 8u : std::min<unsigned int>(grid.x, ctx->smCount * 16u);  // few warps end with an atomic
+    if (cluster) grid.y = 1;
+    withForm(f, [&](auto n, auto x) {
+        if (cluster) {
+            launchNext(ctx, mxTopClusterKernel<T, WIDE, decltype(n)::value, decltype(x)::value>, grid, block, 8, p);
+        } else {
+            launchNext(ctx, mxTopKernel<T, WIDE, decltype(n)::value, decltype(x)::value>, grid, block, 1, p);
+        }
+    });
 }
 
-template <class T, bool NV, bool WIDE, int UNITS>
-void launchQuant(Context* ctx, const MxQuantParams& p, long long units) {
+template <class T, bool NV, bool WIDE>
+void quantizeWith(Context* ctx, const MxQuantParams& p) {
+    if (NV && p.scaleFrom == kScaleFound) findTop<T, WIDE>(ctx, p);
+    // an empty matrix has no scales, but its factor is still written
+    const long long units = std::max((p.cols + 31) / 32 * 4, p.scaleBlocks * (NV ? 2 : 4));
+    if ((p.rows == 0 || units == 0) && !(NV && p.scaleFrom != kScaleGiven)) return;
+    const Form f = formFor(ctx, p.rows, units);
     dim3 grid, block;
-    gridFor(p.rows, units, UNITS, &grid, &block);
+    gridFor(p.rows, f.x, f.fixed ? 128 : 256, static_cast<long long>(f.x) * f.units, units, &grid, &block);
     const int rowCtas = static_cast<int>(grid.x);
     if (p.scaleRows > p.rows) {
         const long long words = (p.scaleRows - p.rows) * (p.scaleBlocks / 4), perX = static_cast<long long>(block.x) * block.y * grid.y;
         grid.x += static_cast<unsigned int>(std::min<long long>((words + perX - 1) / perX, 1024));
     }
-    if (p.values) {
-        launchNext(ctx, mxQuantKernel<T, NV, WIDE, true, UNITS>, grid, block, p, rowCtas);
-    } else {
-        launchNext(ctx, mxQuantKernel<T, NV, WIDE, false, UNITS>, grid, block, p, rowCtas);
-    }
-}
-
-template <class T, bool WIDE, int UNITS>
-void launchTop(Context* ctx, const MxQuantParams& p) {
-    dim3 grid, block;
-    gridFor(p.rows, (p.cols + 7) / 8, UNITS, &grid, &block);
-    grid.x = std::min<unsigned int>(grid.x, ctx->smCount * 16u);  // few warps end with an atomic
-    launchNext(ctx, mxTopKernel<T, WIDE, UNITS>, grid, block, p);
-}
-
-template <class T, bool WIDE, int UNITS>
-void quantizeWith(Context* ctx, const MxQuantParams& p, bool nv) {
-    if (nv && p.scaleFrom == kScaleFound) {
-        fillBytes(ctx, p.tensorScale, 0, 8);
-        if (p.rows > 0 && p.cols > 0) launchTop<T, WIDE, UNITS>(ctx, p);
-    }
-    // an empty matrix has no scales, but its factor is still written
-    const long long units = std::max((p.cols + 31) / 32 * 4, p.scaleBlocks * (nv ? 2 : 4));
-    if ((p.rows == 0 || units == 0) && !(nv && p.scaleFrom != kScaleGiven)) return;
-    if (nv) {
-        launchQuant<T, true, WIDE, UNITS>(ctx, p, units);
-    } else {
-        launchQuant<T, false, WIDE, UNITS>(ctx, p, units);
-    }
+    withForm(f, [&](auto n, auto x) {
+        if (p.values) {
+            launchNext(ctx, mxQuantKernel<T, NV, WIDE, true, decltype(n)::value, decltype(x)::value>, grid, block, 1, p, rowCtas);
+        } else {
+            launchNext(ctx, mxQuantKernel<T, NV, WIDE, false, decltype(n)::value, decltype(x)::value>, grid, block, 1, p, rowCtas);
+        }
+    });
 }
 
 template <class T>
 void quantizeAs(Context* ctx, const MxQuantParams& p, bool nv) {
     // eight columns at a time, all of them there: 16-byte accesses
     const bool wide = p.cols % 8 == 0 && aligned16(p.src, p.srcLd * sizeof(T)) && (!p.values || aligned16(p.values, p.valuesLd * sizeof(T)));
-    if (!longRows(ctx, p.rows, p.cols / 8)) {
-        wide ? quantizeWith<T, true, 1>(ctx, p, nv) : quantizeWith<T, false, 1>(ctx, p, nv);
+    if (nv) {
+        wide ? quantizeWith<T, true, true>(ctx, p) : quantizeWith<T, true, false>(ctx, p);
     } else {
-        wide ? quantizeWith<T, true, kUnits>(ctx, p, nv) : quantizeWith<T, false, kUnits>(ctx, p, nv);
+        wide ? quantizeWith<T, false, true>(ctx, p) : quantizeWith<T, false, false>(ctx, p);
     }
 }
 
-template <class T, int UNITS>
-void dequantizeWith(Context* ctx, const MxDequantParams& p, bool nv) {
+template <class T, bool NV, bool WIDE>
+void dequantizeWith(Context* ctx, const MxDequantParams& p) {
+    const long long units = (p.cols + 7) / 8;
+    const Form f = formFor(ctx, p.rows, units);
     dim3 grid, block;
-    gridFor(p.rows, (p.cols + 7) / 8, UNITS, &grid, &block);
-    const bool wide = p.cols % 8 == 0 && aligned16(p.out, p.outLd * sizeof(T));
-    if (nv && wide) {
-        launchNext(ctx, mxDequantKernel<T, true, true, UNITS>, grid, block, p);
-    } else if (nv) {
-        launchNext(ctx, mxDequantKernel<T, true, false, UNITS>, grid, block, p);
-    } else if (wide) {
-        launchNext(ctx, mxDequantKernel<T, false, true, UNITS>, grid, block, p);
-    } else {
-        launchNext(ctx, mxDequantKernel<T, false, false, UNITS>, grid, block, p);
-    }
+    gridFor(p.rows, f.x, f.fixed ? 128 : 256, static_cast<long long>(f.x) * f.units, units, &grid, &block);
+    withForm(f, [&](auto n, auto x) {
+        launchNext(ctx, mxDequantKernel<T, NV, WIDE, decltype(n)::value, decltype(x)::value>, grid, block, 1, p);
+    });
 }
 
 template <class T>
 void dequantizeAs(Context* ctx, const MxDequantParams& p, bool nv) {
-    if (!longRows(ctx, p.rows, p.cols / 8)) {
-        dequantizeWith<T, 1>(ctx, p, nv);
+    const bool wide = p.cols % 8 == 0 && aligned16(p.out, p.outLd * sizeof(T));
+    if (nv) {
+        wide ? dequantizeWith<T, true, true>(ctx, p) : dequantizeWith<T, true, false>(ctx, p);
     } else {
-        dequantizeWith<T, kUnits>(ctx, p, nv);
+        wide ? dequantizeWith<T, false, true>(ctx, p) : dequantizeWith<T, false, false>(ctx, p);
     }
 }
 

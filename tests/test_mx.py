@@ -183,10 +183,11 @@ def test_quantize(dev, fmt, dtype, rows, cols):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("fmt,dtype,cols", [(A.NVFP4, A.BF16, 4099), (A.MXFP4, A.F32, 4096), (A.NVFP4, A.F16, 4128), (A.MXFP4, A.F16, 3999)])
-def test_large_matrices(dev, fmt, dtype, cols):
+@pytest.mark.parametrize("fmt,dtype,rows,cols", [(A.NVFP4, A.BF16, 1300, 4099), (A.MXFP4, A.F32, 1300, 4096), (A.NVFP4, A.F16, 1300, 4128),
+                                                 (A.MXFP4, A.F16, 1300, 3999), (A.NVFP4, A.F32, 20000, 250), (A.NVFP4, A.BF16, 40000, 130),
+                                                 (A.MXFP4, A.BF16, 9001, 600)])
+def test_large_matrices(dev, fmt, dtype, rows, cols):
     """Enough rows for the kernels' form with several pieces of a row per thread, aligned and not, and back."""
-    rows = 1300
     x = awkward(rows, cols, dtype, cols)
     q = O.quantize(x.double().numpy(), fmt)
     want = torch.from_numpy(q["values"].astype(np.float32)).to(x.dtype).nan_to_num(nan=12345.0)
