@@ -143,16 +143,29 @@ __device__ __forceinline__ Raw<T> load8(const T* p, int left) {
 // a row hold bytes of others, too: they are read, never written whole -- a line that holds one byte of a matrix lies in
 // the same allocation as that byte.
 //
-// N words, `bytes` (0 .. 15) on from the start of z
+// N words, `bytes` (0 .. 15) on from the start of z.  A branch, since a warp's threads mostly have one row's `bytes`:
+// picking the words one by one costs more than the rest.
 template <int N>
 __device__ __forceinline__ void shifted(const unsigned int z[N + 4], unsigned int bytes, unsigned int out[N]) {
-    unsigned int a[N + 2], b[N + 1];
+    const unsigned int bits = (bytes & 3) * 8;
+    switch (bytes >> 2) {
+    case 0:
 #pragma unroll
-    for (int i = 0; i < N + 2; ++i) a[i] = bytes & 8 ? z[i + 2] : z[i];
+        for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(z[i], z[i + 1], bits);
+        break;
+    case 1:
 #pragma unroll
-    for (int i = 0; i < N + 1; ++i) b[i] = bytes & 4 ? a[i + 1] : a[i];
+        for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(z[i + 1], z[i + 2], bits);
+        break;
+    case 2:
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(b[i], b[i + 1], (bytes & 3) * 8);
+        for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(z[i + 2], z[i + 3], bits);
+        break;
+    default:
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = __funnelshift_r(z[i + 3], z[i + 4], bits);
+        break;
+    }
 }
 // hasNext: the next thread of the warp has the next eight elements of the row.  Whole warps call this.
 template <class T>
@@ -161,18 +174,22 @@ __device__ __forceinline__ Raw<T> loadAny(const T* p, int left, bool hasNext) {
     const unsigned int m = static_cast<unsigned int>(reinterpret_cast<uintptr_t>(p) & 15);
     const uint4* line = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - m);
     const int valid = min(max(left, 0), 8) * static_cast<int>(sizeof(T));
+    uint4 l[n];
+    if (left >= 8) {
+#pragma unroll
+        for (int k = 0; k < n; ++k) l[k] = __ldcs(line + k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < n; ++k) l[k] = valid > 0 && static_cast<int>(m) + valid > 16 * k ? __ldcs(line + k) : make_uint4(0, 0, 0, 0);
+    }
     unsigned int w[4 * n + 4];
 #pragma unroll
-    for (int k = 0; k < n; ++k) {
-        uint4 l = make_uint4(0, 0, 0, 0);
-        if (valid > 0 && static_cast<int>(m) + valid > 16 * k) l = __ldcs(line + k);
-        w[4 * k] = l.x, w[4 * k + 1] = l.y, w[4 * k + 2] = l.z, w[4 * k + 3] = l.w;
-    }
+    for (int k = 0; k < n; ++k) w[4 * k] = l[k].x, w[4 * k + 1] = l[k].y, w[4 * k + 2] = l[k].z, w[4 * k + 3] = l[k].w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[4 * n + i] = __shfl_down_sync(0xFFFFFFFFu, w[i], 1);
     if ((!hasNext || left <= 8) && static_cast<int>(m) + valid > 16 * n) {
-        const uint4 l = __ldcs(line + n);
-        w[4 * n] = l.x, w[4 * n + 1] = l.y, w[4 * n + 2] = l.z, w[4 * n + 3] = l.w;
+        const uint4 next = __ldcs(line + n);
+        w[4 * n] = next.x, w[4 * n + 1] = next.y, w[4 * n + 2] = next.z, w[4 * n + 3] = next.w;
     }
     Raw<T> r;
     shifted<4 * n>(w, m, reinterpret_cast<unsigned int*>(r.v));
@@ -197,14 +214,24 @@ __device__ __forceinline__ void storeAny(T* p, int left, const T t[8], bool hasP
     for (int i = 0; i < 4 * n; ++i) z[4 + i] = v[i];
     shifted<4 * n>(z, (16 - m) & 15, o);
     uint4* line = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - m);
-    // the bytes of this thread's that lines take: from the start, or the second line if the first one has others' bytes
-    int from = m == 0 || hasPrev ? 0 : 16 - m, to = from;
+    if (m == 0) {
 #pragma unroll
-    for (int k = 0; k < n; ++k) {
-        if (valid >= 16 * (k + 1) - m && (k > 0 || from == 0)) {
-            __stcs(line + k, m == 0 ? make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3])
-                                    : make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
-            to = 16 * (k + 1) - m;
+        for (int i = 0; i < 4 * n; ++i) o[i] = v[i];
+    }
+    // the bytes of this thread's that lines take: from the start, or the second line if the first one has others' bytes
+    const int from = m == 0 || hasPrev ? 0 : 16 - m;
+    int to = from;
+    if (left >= 8 && from == 0) {
+#pragma unroll
+        for (int k = 0; k < n; ++k) __stcs(line + k, make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+        to = 16 * n - m;
+    } else {
+#pragma unroll
+        for (int k = 0; k < n; ++k) {
+            if (valid >= 16 * (k + 1) - m && (k > 0 || from == 0)) {
+                __stcs(line + k, make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+                to = 16 * (k + 1) - m;
+            }
         }
     }
     // the next thread's first line takes the last m bytes, if it is written whole
