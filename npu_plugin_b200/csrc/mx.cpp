@@ -129,6 +129,8 @@ void mxCheckMatmul(const b200c_mx_matrix* a, const b200c_mx_matrix* b, const voi
     if (a->scale_layout != B200C_MX_SCALES_TILED || b->scale_layout != B200C_MX_SCALES_TILED) {
         throw BadArg("the product reads tiled scales");
     }
+    // the loads' descriptors hold distances below 2^40 bytes
+    if (a->ld >= (int64_t(1) << 40) || b->ld >= (int64_t(1) << 40)) throw BadArg("the distance between rows of codes is too large for a product");
     const Range dst = checkDense("output", out, dtype, a->rows, b->rows, outLd);
     for (const MatrixRanges* m : {&ra, &rb}) {
         checkApart(dst, m->codes);

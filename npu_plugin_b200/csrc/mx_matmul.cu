@@ -1005,7 +1005,7 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     g.out = out;
     g.ld = outLd;
     g.outTag = dtype == B200C_F16 ? T_F16 : dtype == B200C_BF16 ? T_BF16 : T_F32;
-    g.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (outLd * es) % 16 == 0;
+    g.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (outLd * es) % 16 == 0 && outLd * es < (int64_t(1) << 40);
     g.err = ctx->errWord;
     if (pairs) {
         if (nv) {

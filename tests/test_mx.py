@@ -290,7 +290,7 @@ def test_empty_matrices(dev):
     (dict(out=0x10000), "overlaps codes"), (dict(out=0x51000), "overlaps scales"), (dict(a=dict(fmt=A.MXFP4)), "different formats"),
     (dict(a=dict(cols=96, ld=48)), "different numbers"), (dict(a=dict(layout=A.MX_SCALES_ROWS)), "tiled scales"),
     (dict(b=dict(layout=A.MX_SCALES_ROWS)), "tiled scales"), (dict(b=dict(tensor_scale=None)), "needs a tensor scale"),
-    (dict(a=dict(codes=0x10001)), "16-byte"), (dict(a=dict(ld=24)), "multiple of 16"),
+    (dict(a=dict(codes=0x10001)), "16-byte"), (dict(a=dict(rows=1, ld=1 << 41), ld=1 << 42, out=1 << 50), "too large for a product"), (dict(a=dict(ld=24)), "multiple of 16"),
 ])
 def test_matmul_refusals(change, said):
     a = matrix(**dict(dict(ld=32), **change.get("a", {})))
@@ -439,3 +439,132 @@ def test_quantise_then_multiply(dev, fmt):
         dx.copy_(x)
         graph.replay()
         check(x)
+
+
+# --------------------------------------------------------------------------- as programs use them together
+@pytest.mark.gpu
+def test_rows_far_apart(dev):
+    """Offsets beyond 2^31 elements and 2^32 bytes: three rows with a gigabyte and more between them."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    rows, cols, far = 3, 70, (1 << 30) + 24
+    x = awkward(rows, cols, A.F16, 1, special=False)
+    for fmt in FORMATS:
+        q = O.quantize(x.double().numpy(), fmt)
+        src = torch.empty(2 * far + cols, dtype=torch.half, device="cuda")
+        view = src.as_strided((rows, cols), (far, 1))
+        view.copy_(x.cuda())
+        ld = (1 << 31) + 32
+        codes = torch.empty(2 * ld + 48, dtype=torch.uint8, device="cuda")
+        scales = torch.empty(mx.sizes(fmt, rows, cols)[2], dtype=torch.uint8, device="cuda")
+        tensor = torch.zeros(2, device="cuda")
+        m = mx.MxMatrix(fmt, rows, cols, codes.data_ptr(), scales.data_ptr(), tensor.data_ptr(), ld=ld)
+        dev.mx_quantize(src.data_ptr(), A.F16, far, m)
+        np.testing.assert_array_equal(codes.as_strided((rows, 48), (ld, 1)).cpu().numpy(), O.pack(q["codes"]))
+        src.as_strided((rows, cols), (far, 1)).zero_()
+        dev.mx_dequantize(m, src.data_ptr(), A.F16, far)
+        np.testing.assert_array_equal(view.cpu().numpy(), q["values"].astype(np.float32).astype(np.float16))
+        out = src.as_strided((rows, rows), (far, 1))
+        dev.mx_matmul(m, m, src.data_ptr(), A.F16, far)
+        check_product(out.double().cpu().numpy(), q["values"], q["values"], A.F16)
+        del src, view, out, codes
+
+
+@pytest.mark.gpu
+def test_two_contexts_on_two_streams_from_two_threads(dev):
+    """Each with its own matrices; the results are those of one after the other."""
+    import threading
+    from npu_plugin_b200.const import CudaBackend
+    shapes = [(40, 3000, 2000), (1600, 1900, 520)]
+    made = []
+    for i, (m, n, k) in enumerate(shapes):
+        a, _ = random_held(A.NVFP4, m, k, i)
+        b, _ = random_held(A.NVFP4, n, k, i + 7)
+        want = torch.empty(m, n, device="cuda")
+        dev.mx_matmul(a.m, b.m, want.data_ptr(), A.F32, n)
+        made.append((a, b, want, torch.empty(m, n, device="cuda")))
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        try:
+            backend = CudaBackend(0)
+            a, b, _, out = made[i]
+            for _ in range(50):
+                backend.mx_matmul(a.m, b.m, out.data_ptr(), A.F32, out.shape[1])
+            backend.synchronize()
+            backend.close()
+        except Exception as e:
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for _, _, want, out in made:
+        assert torch.equal(want, out)
+
+
+@pytest.mark.gpu
+def test_two_graphs_in_turn_and_every_result_the_same_bytes(dev):
+    """Two captured layers that share their weights, replayed in turn, against eager runs."""
+    n, k = 700, 1100
+    w, _ = random_held(A.MXFP4, n, k, 3)
+    cases = []
+    for m in (3, 150):
+        g = torch.Generator().manual_seed(m)
+        x = torch.randn(m, k, generator=g).bfloat16().cuda()
+        h = Held(A.MXFP4, m, k, A.MX_SCALES_TILED)
+        out = torch.zeros(m, n, device="cuda")
+
+        def step(x=x, h=h, out=out):
+            dev.mx_quantize(x.data_ptr(), A.BF16, k, h.m)
+            dev.mx_matmul(h.m, w.m, out.data_ptr(), A.F32, n)
+        step()
+        torch.cuda.synchronize()
+        want = out.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dev.set_stream(torch.cuda.current_stream().cuda_stream)
+            step()
+        dev.set_stream(torch.cuda.current_stream().cuda_stream)
+        cases.append((graph, out, want, x, h))  # the graph reads x and writes h: they have to live as long
+    for _ in range(20):
+        for graph, out, *_ in cases:
+            out.zero_()
+            graph.replay()
+        for _, out, want, *_ in cases:
+            assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_first_use_inside_a_capture():
+    """A process whose very first calls are captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from npu_plugin_b200 import _cabi as A, const, mx
+b = const.CudaBackend(0)
+x = torch.randn(300, 640, device="cuda").half()
+out = torch.zeros(300, 300, device="cuda")
+ld, nc, ns = mx.sizes(A.NVFP4, 300, 640)
+codes, scales, t = (torch.empty(n, dtype=torch.uint8, device="cuda") for n in (nc, ns, 8))
+m = mx.MxMatrix(A.NVFP4, 300, 640, codes.data_ptr(), scales.data_ptr(), t.data_ptr())
+back = torch.empty_like(x)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b.set_stream(torch.cuda.current_stream().cuda_stream)
+    b.mx_quantize(x.data_ptr(), A.F16, 640, m)
+    b.mx_dequantize(m, back.data_ptr(), A.F16, 640)
+    b.mx_matmul(m, m, out.data_ptr(), A.F32, 300)
+g.replay()
+torch.cuda.synchronize()
+v = back.double()
+assert (out.double() - v @ v.t()).abs().max() < 1e-3 * 640
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
