@@ -128,12 +128,17 @@ struct Raw {
     static constexpr int n = 8 * sizeof(T) / 16;
     uint4 v[n];
 };
+// A line of 16 bytes; KEEP: it will be read again, and should stay in L2
+template <bool KEEP>
+__device__ __forceinline__ uint4 loadLine(const uint4* p) {
+    return KEEP ? __ldg(p) : __ldcs(p);
+}
 // 16-byte loads that are aligned: all eight are there, or none
-template <class T>
+template <class T, bool KEEP>
 __device__ __forceinline__ Raw<T> load8(const T* p, int left) {
     Raw<T> r;
 #pragma unroll
-    for (int i = 0; i < Raw<T>::n; ++i) r.v[i] = left > 0 ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < Raw<T>::n; ++i) r.v[i] = left > 0 ? loadLine<KEEP>(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
     return r;
 }
 
@@ -168,7 +173,7 @@ __device__ __forceinline__ void shifted(const unsigned int z[N + 4], unsigned in
     }
 }
 // hasNext: the next thread of the warp has the next eight elements of the row.  Whole warps call this.
-template <class T>
+template <class T, bool KEEP>
 __device__ __forceinline__ Raw<T> loadAny(const T* p, int left, bool hasNext) {
     constexpr int n = Raw<T>::n;
     const unsigned int m = static_cast<unsigned int>(reinterpret_cast<uintptr_t>(p) & 15);
@@ -177,10 +182,10 @@ __device__ __forceinline__ Raw<T> loadAny(const T* p, int left, bool hasNext) {
     uint4 l[n];
     if (left >= 8) {
 #pragma unroll
-        for (int k = 0; k < n; ++k) l[k] = __ldcs(line + k);
+        for (int k = 0; k < n; ++k) l[k] = loadLine<KEEP>(line + k);
     } else {
 #pragma unroll
-        for (int k = 0; k < n; ++k) l[k] = valid > 0 && static_cast<int>(m) + valid > 16 * k ? __ldcs(line + k) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < n; ++k) l[k] = valid > 0 && static_cast<int>(m) + valid > 16 * k ? loadLine<KEEP>(line + k) : make_uint4(0, 0, 0, 0);
     }
     unsigned int w[4 * n + 4];
 #pragma unroll
@@ -188,7 +193,7 @@ __device__ __forceinline__ Raw<T> loadAny(const T* p, int left, bool hasNext) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[4 * n + i] = __shfl_down_sync(0xFFFFFFFFu, w[i], 1);
     if ((!hasNext || left <= 8) && static_cast<int>(m) + valid > 16 * n) {
-        const uint4 next = __ldcs(line + n);
+        const uint4 next = loadLine<KEEP>(line + n);
         w[4 * n] = next.x, w[4 * n + 1] = next.y, w[4 * n + 2] = next.z, w[4 * n + 3] = next.w;
     }
     Raw<T> r;
@@ -364,7 +369,7 @@ __device__ __forceinline__ unsigned int topOf(const MxQuantParams& p, int lane) 
                 const long long r = r0 + (UNITS > 1 ? 0 : i * step) + (x < 32 ? lane / x : 0);
                 const T* from = static_cast<const T*>(p.src) + r * p.srcLd + ui * 8ll;
                 const int left = r < p.rows ? cols - 8 * ui : 0;
-                raw[i] = WIDE ? load8<T>(from, left) : loadAny<T>(from, left, hasNext);
+                raw[i] = WIDE ? load8<T, true>(from, left) : loadAny<T, true>(from, left, hasNext);
             }
 #pragma unroll
             for (int i = 0; i < UNITS * rows; ++i) top = topFinite<T>(top, raw[i]);
@@ -373,13 +378,25 @@ __device__ __forceinline__ unsigned int topOf(const MxQuantParams& p, int lane) 
     return __reduce_max_sync(0xFFFFFFFFu, top);
 }
 
+// A memset in the stream would end the kernels' overlapping: 3 us more.
+__global__ void mxZeroKernel(float* tensorScale) {
+    afterLast();
+    if (threadIdx.x < 2) tensorScale[threadIdx.x] = 0.f;
+}
+
 // -> tensorScale[1], zeroed before.  A maximum does not depend on the order it is taken in.
 template <class T, bool WIDE, int UNITS, int X>
 __global__ void __launch_bounds__(256) mxTopKernel(const __grid_constant__ MxQuantParams p) {
+    __shared__ unsigned int tops[8];
     afterLast();
-    const int lane = (threadIdx.y * Lay<UNITS, X>::x() + threadIdx.x) & 31;
-    const unsigned int top = topOf<T, WIDE, UNITS, X>(p, lane);
-    if (lane == 0 && top) atomicMax(reinterpret_cast<unsigned int*>(p.tensorScale) + 1, top);
+    const int thread = threadIdx.y * Lay<UNITS, X>::x() + threadIdx.x, lane = thread & 31, warps = blockDim.x * blockDim.y / 32;
+    unsigned int top = topOf<T, WIDE, UNITS, X>(p, lane);
+    if (lane == 0) tops[thread >> 5] = top;
+    __syncthreads();
+    if (thread < 32) {
+        top = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? tops[lane] : 0u);
+        if (lane == 0 && top) atomicMax(reinterpret_cast<unsigned int*>(p.tensorScale) + 1, top);
+    }
 }
 
 // One cluster of CTAs: its first one collects the others' results, and nothing has to be zeroed before.
@@ -420,7 +437,7 @@ __device__ __forceinline__ unsigned int topHere(const MxQuantParams& p, int thre
             const int at = first + i * threads, r = at / across, c = at - r * across;
             const T* from = static_cast<const T*>(p.src) + r * p.srcLd + c * each;
             if (WIDE) {
-                raw[i] = load8<T>(from, at < n ? 8 : 0);
+                raw[i] = load8<T, true>(from, at < n ? 8 : 0);
             } else {
                 reinterpret_cast<T*>(raw)[i] = at < n ? *from : fromFloat<T>(0.f);
             }
@@ -551,7 +568,7 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
     const int cols = static_cast<int>(p.cols), units = (cols + 31) / 32 * 4;
     const int all = max(units, static_cast<int>(p.scaleBlocks) * lanes);  // those of a tile's filling scales too
     // from the last row to the first: where the largest magnitude was looked for just before, the last rows are
-    // what L2 still holds
+    // what L2 still holds (11008 x 4096 f16: 65.6 -> 62.5 us for both kernels)
     const long long r = p.rows - 1 - (static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y);
     const int run = min(x, 32);  // threads of a warp that lie in one row
     const bool hasPrev = (lane & (run - 1)) != 0, hasNext = (lane & (run - 1)) != run - 1;
@@ -568,7 +585,7 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
         for (int i = 0; i < UNITS; ++i) {
             const T* from = src + u * 8ll + i * x * 8;
             const int left = r >= 0 ? cols - 8 * (u + i * x) : 0;
-            raw[i] = WIDE ? load8<T>(from, left) : loadAny<T>(from, left, hasNext);
+            raw[i] = WIDE ? load8<T, false>(from, left) : loadAny<T, false>(from, left, hasNext);
         }
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
@@ -713,8 +730,10 @@ void findTop(Context* ctx, const MxQuantParams& p) {
     gridFor(p.rows, f.x, f.fixed ? 128 : 256, static_cast<long long>(f.x) * f.units, units, &grid, &block);
     // eight CTAs read about 1 MB in the time that zeroing the word and a grid's atomics take
     const bool cluster = p.rows * units * 8 * static_cast<long long>(sizeof(T)) <= (1ll << 20);
-    if (!cluster) fillBytes(ctx, p.tensorScale, 0, 8);
-    grid.x = cluster ? 8u : std::min<unsigned int>(grid.x, ctx->smCount * 16u);  // few warps end with an atomic
+    if (!cluster) launchNext(ctx, mxZeroKernel, dim3(1), dim3(32), 1, p.tensorScale);
+    // all atomics go to one word, one after another: one for each of few CTAs (one for each warp of many took 16 us for
+    // 1024 x 4096)
+    grid.x = cluster ? 8u : std::min<unsigned int>(grid.x, ctx->smCount * (f.fixed ? 8u : 4u));
     if (cluster) grid.y = 1;
     withForm(f, [&](auto n, auto x) {
         if (cluster) {
