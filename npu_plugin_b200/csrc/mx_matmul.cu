@@ -4,6 +4,13 @@
 // sum_k A[i][k] B[j][k] with A[i][k] = code * scale: tcgen05.mma takes the codes from shared memory and the
 // scales from tensor memory and multiplies both in, 64 elements of k at a time; sums are 32 bits wide.
 // One side's rows are the 128 rows of a tile ("P"), the other's its columns ("Q").
+//
+// Two kernels.  mxMatmulPairKernel, for products of many tiles, is bound by the tensor pipe, and by power where it
+// runs long: 8192 x 4096 x 11008 (nvfp4) 124 us, 5.96 PFLOP/s -- 150 us in a long run, at 1000 W and 1.38 GHz.  Its tile of 256 x 256 for
+// two SMs is what the way from L2 allows: an SM takes 64 bytes a clock, and a 128 x 256 tile of one SM would need
+// 54 KB for 512 clocks of products, this one 38 KB.  mxMatmulKernel, for few rows on the left, is bound by that way from L2
+// and by latency: 1 x 11008 x 4096 (nvfp4) 6.4 us, 16 x 4096 x 11008 (mxfp4) 6.4 us, and with weights from DRAM
+// 1 x 32000 x 11008 30.8 us, 93 % of the copy rate.
 #include "mx.h"
 #include "runtime.h"
 
@@ -27,7 +34,6 @@ struct MxMatmulParams {
     const float* tensorQ;
     long long rowsP, rowsQ, k;
     long long chunks;      // tiles of 4 blocks along k: 512 bytes of scales each, per 128 rows
-    int scaleTilesQ;       // tiles of 128 rows that the Q side's scales have
     int ktiles;
     int tilesP, tilesQ;
     int split;             // CTAs that share a tile's k
@@ -312,8 +318,8 @@ __device__ __forceinline__ float toOut<float>(float v) {
     return v;
 }
 
-// The single-CTA kernel's P is the right matrix: N accumulator columns of lane p are N rows of the product at column p, and
-// a warp's lanes store 32 neighbours at a time.
+// The single-CTA kernel's P is the right matrix: N accumulator columns of lane p are N rows of the product at
+// column p, and a warp's lanes store 32 neighbours at a time.
 template <class T, int N>
 __device__ __forceinline__ void storeAcross(const MxMatmulParams& g, long long p, long long q0, const float* v) {
     if (p >= g.rowsP) return;
@@ -345,9 +351,10 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
     }
 }
 
-// A tile whose k is shared out: its sums lie
-// in `split` (at most MOST) CTAs' shared memory as [BN][128]; this CTA adds up its share of the columns, in the order of the ranks.  A thread takes four rows at a time, and 16 loads from the cluster's memory
-// are under way at once: with one column at a time the waiting for them took longer than the product itself.
+// A tile whose k is shared out: its sums lie in `split` (at most MOST) CTAs' shared memory as [BN][128]; this CTA adds
+// up its share of the columns, in the order of the ranks, so that the result is the same on every run.  A thread takes
+// four rows at a time, and 16 loads from the cluster's memory are under way at once: with one column at a time the
+// waiting for them took longer than the product itself.
 template <class T, int BN, int MOST>
 __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0,
                                             long long q0, float alpha) {
@@ -984,6 +991,8 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
                                   ctx->stream));
         return;
     }
+    // pairs from a quarter of the SMs in tiles on: 512 x 4096 x 4096 (32 tiles) takes 8.8 us by single CTAs and 9.9 by
+    // pairs, 768 (48 tiles) 10.9 and 10.4
     const long long big = ((a.rows + 255) / 256) * ((b.rows + 255) / 256);
     const bool pairs = big >= ctx->smCount / 4 && a.rows > 128 && b.rows > 128;
     const b200c_mx_matrix& p = pairs ? a : b;
@@ -998,7 +1007,6 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     g.rowsQ = q.rows;
     g.k = a.cols;
     g.chunks = (mxBlocks(a.format, a.cols) + 3) / 4;
-    g.scaleTilesQ = static_cast<int>((q.rows + 127) / 128);
     g.ktiles = static_cast<int>((a.cols + kTileK - 1) / kTileK);
     g.tilesP = g.tilesQ = 0;
     g.split = 1;
