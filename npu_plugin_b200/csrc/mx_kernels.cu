@@ -491,8 +491,9 @@ struct Divisor {
         r = __fmaf_rn(__fmaf_rn(-d, r0, 1.f), r0, r0);
     }
     __device__ __forceinline__ float near(float v) const {
+        // the remainder is taken with its sign turned: the other way round -0 would become 0
         const float q = __fmul_rn(v, r);
-        return copysignf(__fmaf_rn(__fmaf_rn(-q, d, v), r, q), v);  // a zero would lose its sign
+        return __fmaf_rn(-__fmaf_rn(q, d, -v), r, q);
     }
     __device__ __forceinline__ float within(float v) const {
         return fminf(fmaxf(v * s1 * s2, -1e30f), 1e30f);
