@@ -5,7 +5,7 @@
 //
 // One pass over the data, bound by DRAM where the values are written, too: 11008 x 4096 f16 to mxfp4 with values
 // 29.9 us (6.85 TB/s of what the pass cannot do without), back to f16 18.5 us (6.2 TB/s).  Without the values it is instruction issue:
-// 23.6 us (4.9 TB/s), and 33.5 us for nvfp4, whose quotients take four instructions an element.
+// 23.6 us (4.9 TB/s), and 30.9 us for nvfp4, whose quotients take three instructions an element.
 #include "mx.h"
 #include "runtime.h"
 
@@ -36,7 +36,12 @@ struct MxQuantParams {
     long long scaleBlocks;  // the same for blocks
 };
 
-enum : int { kScaleGiven, kScaleFound /* tensorScale[1] holds the largest magnitude */, kScaleHere /* the kernel looks for it */ };
+enum : int {
+    kScaleGiven,
+    kScaleFound,    // tensorScale[1] holds the largest magnitude
+    kScaleHere,     // the kernel looks for it first
+    kScaleGuessed,  // tensorScale[0] is that of some of the rows; the kernel finds tensorScale[1] on its way
+};
 
 struct MxDequantParams {
     const unsigned char* codes;
@@ -434,7 +439,11 @@ __global__ void __launch_bounds__(256) mxTopClusterKernel(const __grid_constant_
             all = max(all, v);
         }
         all = __reduce_max_sync(0xFFFFFFFFu, all);
-        if (lane == 0) p.tensorScale[1] = __uint_as_float(all);
+        if (lane == 0) {
+            // for a guess; of zeros the smallest that there is: that of the whole matrix may be any
+            p.tensorScale[0] = all ? tensorScaleOf(__uint_as_float(all)) : 1.17549435e-38f;
+            p.tensorScale[1] = __uint_as_float(all);
+        }
     }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
     }
     float t = 1.f;
     if (NV) {
-        if (p.scaleFrom == kScaleGiven) {
+        if (p.scaleFrom == kScaleGiven || p.scaleFrom == kScaleGuessed) {
             t = p.tensorScale[0];
         } else {
             float top;
@@ -594,6 +603,8 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
     T* values = static_cast<T*>(p.values) + r * p.valuesLd;
     // tiled: blocks of four lie 512 bytes apart
     unsigned char* scales = p.scales + (r >= 0 ? scaleAt(p.tiled, r, 0, p.blocks) : 0);
+    const bool watch = NV && p.scaleFrom == kScaleGuessed;
+    unsigned int seen = 0;  // the largest finite magnitude
     const int begin = L::firstUnit() - static_cast<int>(threadIdx.x);
     for (int base = begin; base < all; base += L::unitStep()) {
         const int u = base + threadIdx.x;
@@ -610,6 +621,7 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
             unsigned int top = top8<T>(raw[i]);
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             if (!NV) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            if (watch) seen = top < 0x7F800000u ? max(seen, top) : topFinite<T>(seen, raw[i]);
             float d;
             unsigned int scale;
             const unsigned int word = encode8<T, NV>(raw[i], top, t, sixT, badT, &scale, &d);
@@ -631,6 +643,108 @@ __global__ void __launch_bounds__(256, 4) mxQuantKernel(const __grid_constant__ 
             }
         }
     }
+    if (watch) {
+        seen = __reduce_max_sync(0xFFFFFFFFu, seen);
+        if (lane == 0) tops[warp] = seen;
+        __syncthreads();
+        if (thread == 0) {
+            for (int i = 1; i < static_cast<int>(blockDim.x * blockDim.y) / 32; ++i) seen = max(seen, tops[i]);
+            unsigned int* word = reinterpret_cast<unsigned int*>(p.tensorScale) + 1;
+            if (seen > *reinterpret_cast<volatile unsigned int*>(word)) atomicMax(word, seen);  // few are
+        }
+    }
+}
+
+// After a guessed factor: where the one that the whole matrix gives is 2^k times it, a block's scale is 2^-k times
+// what was stored, with the same codes and values, as long as neither is at the ends of what e4m3 holds: between them
+// its rounding is relative to the number.  The guess is that of some of the rows, so k > 0; a scale of 0 then stays 0
+// and NaN stays NaN.  The blocks at the ends, mostly few, are quantised again.  Scales are walked in the order that
+// they are stored in: row by row, tiled ones took 122 us (32000 x 4096) for sectors of which a warp used four bytes.
+template <class T>
+__global__ void __launch_bounds__(256) mxRepairKernel(const __grid_constant__ MxQuantParams p) {
+    afterLast();
+    const float guess = p.tensorScale[0], t = tensorScaleOf(p.tensorScale[1]);
+    if (t == guess) return;
+    const int k = static_cast<int>(__float_as_uint(t) >> 23) - static_cast<int>(__float_as_uint(guess) >> 23);
+    const Divisor sixT(6.f * t, 0.f);
+    const int lane = threadIdx.x & 31;
+    const long long n = p.scaleRows * p.scaleBlocks;
+    const int each = reinterpret_cast<uintptr_t>(p.scales) % 16 == 0 ? 16 : 1;  // scales of a thread
+    const long long step = static_cast<long long>(gridDim.x) * blockDim.x * each;
+    // whole warps go through the loop together
+    for (long long at = (static_cast<long long>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31)) * each; at < n; at += step) {
+        const long long mine = at + lane * each;
+        const int count = static_cast<int>(max(0ll, min(static_cast<long long>(each), n - mine)));
+        alignas(16) unsigned char s[16];
+        if (count == 16) {
+            *reinterpret_cast<uint4*>(s) = *reinterpret_cast<const uint4*>(p.scales + mine);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = j < count ? p.scales[mine + j] : 0;
+        }
+        unsigned int again = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int b = s[j], moved = b - 8 * k;
+            if (b != 0 && b != 0x7F) {
+                if (b < 8 || b > 125 || moved < 8) {
+                    again |= 1u << j;
+                } else {
+                    s[j] = static_cast<unsigned char>(moved);
+                }
+            }
+        }
+        if (count == 16) {
+            *reinterpret_cast<uint4*>(p.scales + mine) = *reinterpret_cast<const uint4*>(s);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < count) p.scales[mine + j] = s[j];
+        }
+        __syncwarp();
+        // one thread's blocks after another's, two threads to each
+        for (unsigned int todo = __ballot_sync(0xFFFFFFFFu, again != 0); todo; todo &= todo - 1) {
+            const int from = __ffs(todo) - 1;
+            const bool on = __shfl_sync(0xFFFFFFFFu, again, from) >> (lane / 2) & 1;
+            const long long i = at + from * each + lane / 2;
+            long long row, b;
+            if (p.tiled) {
+                const long long tile = i / 512, chunks = p.scaleBlocks / 4;
+                const int in = static_cast<int>(i % 512);
+                row = tile / chunks * 128 + in % 16 / 4 * 32 + in / 16;
+                b = tile % chunks * 4 + in % 4;
+            } else {
+                row = i / p.blocks;
+                b = i % p.blocks;
+            }
+            const long long u = b * 2 + (lane & 1);  // eight elements
+            const int left = on ? static_cast<int>(min(8ll, p.cols - 8 * u)) : 0;
+            Raw<T> raw;
+            T* e = reinterpret_cast<T*>(raw.v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = j < left ? static_cast<const T*>(p.src)[row * p.srcLd + u * 8 + j] : fromFloat<T>(0.f);
+            unsigned int top = top8<T>(raw);
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            float d;
+            unsigned int scale;
+            const unsigned int word = encode8<T, true>(raw, top, t, sixT, false, &scale, &d);
+            if (left > 0) {
+                if ((lane & 1) == 0) p.scales[i] = static_cast<unsigned char>(scale);
+                *reinterpret_cast<unsigned int*>(p.codes + row * p.ld + u * 4) = word;
+                if (p.values) {
+                    alignas(16) T w[8];
+                    values8<T, false>(word, d, w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < left) static_cast<T*>(p.values)[row * p.valuesLd + u * 8 + j] = w[j];
+                }
+            }
+        }
+    }
+}
+__global__ void mxScaleKernel(float* tensorScale) {
+    afterLast();
+    if (threadIdx.x == 0) tensorScale[0] = tensorScaleOf(tensorScale[1]);
 }
 
 template <class T, bool NV, bool WIDE, int UNITS, int X>
@@ -740,7 +854,7 @@ bool aligned16(const void* p, long long ldBytes) {
 }
 
 template <class T, bool WIDE>
-void findTop(Context* ctx, const MxQuantParams& p) {
+void findTop(Context* ctx, const MxQuantParams& p) {  // -> tensorScale[1]; of up to 1 MB [0] as well
     const long long units = (p.cols + 7) / 8;
     const Form f = formFor(ctx, p.rows, units);
     dim3 grid, block;
@@ -764,6 +878,13 @@ void findTop(Context* ctx, const MxQuantParams& p) {
 template <class T, bool NV, bool WIDE>
 void quantizeWith(Context* ctx, const MxQuantParams& p) {
     if (NV && p.scaleFrom == kScaleFound) findTop<T, WIDE>(ctx, p);
+    if (NV && p.scaleFrom == kScaleGuessed) {
+        MxQuantParams some = p;  // rows far from one another, less than 1 MB in all
+        const long long every = (p.rows * ((p.cols + 7) / 8 * 8) * static_cast<long long>(sizeof(T)) >> 20) + 1;
+        some.rows = std::max<long long>(1, p.rows / every);
+        some.srcLd = p.srcLd * every;
+        findTop<T, WIDE>(ctx, some);
+    }
     // an empty matrix has no scales, but its factor is still written
     const long long units = std::max((p.cols + 31) / 32 * 4, p.scaleBlocks * (NV ? 2 : 4));
     if ((p.rows == 0 || units == 0) && !(NV && p.scaleFrom != kScaleGiven)) return;
@@ -782,6 +903,10 @@ void quantizeWith(Context* ctx, const MxQuantParams& p) {
             launchNext(ctx, mxQuantKernel<T, NV, WIDE, false, decltype(n)::value, decltype(x)::value>, grid, block, 1, p, rowCtas);
         }
     });
+    if (NV && p.scaleFrom == kScaleGuessed) {
+        launchNext(ctx, mxRepairKernel<T>, dim3(ctx->smCount * 8u), dim3(256), 1, p);
+        launchNext(ctx, mxScaleKernel, dim3(1), dim3(32), 1, p.tensorScale);
+    }
 }
 
 template <class T>
@@ -830,9 +955,16 @@ void launchMxQuantize(Context* ctx, const void* src, int dtype, int64_t srcLd, c
     p.scales = static_cast<unsigned char*>(out.scales);
     p.tiled = out.scale_layout == B200C_MX_SCALES_TILED;
     p.tensorScale = out.tensor_scale;
-    // up to 64 KB every CTA looks the matrix through by itself: 16 loads of a thread, where two launches before this
-    // one take about 5 us
-    p.scaleFrom = scaleGiven ? kScaleGiven : out.rows * ((out.cols + 7) / 8 * 8) * (dtBits(dtype) / 8) <= 65536 ? kScaleHere : kScaleFound;
+    // Up to 64 KB every CTA looks the matrix through by itself: 16 loads of a thread, where two launches before this
+    // one take about 5 us.  From 128 MB on, when most of the second read would not come from L2 either, the matrix is
+    // read once, with a guess that is put right afterwards (f32 with values, 32000 x 4096: 275 -> 196 us, 8192 x 8192:
+    // 141 -> 99; f16 of 64 MB: 40 -> 47 us, of 90 MB: 56 -> 58).  The guess looks at whole rows, so they are at most a
+    // quarter of what it may read.
+    const int64_t bytes = out.rows * ((out.cols + 7) / 8 * 8) * (dtBits(dtype) / 8);
+    p.scaleFrom = scaleGiven                                                       ? kScaleGiven
+                  : bytes <= 65536                                                 ? kScaleHere
+                  : bytes >= (128ll << 20) && out.cols * (dtBits(dtype) / 8) <= (1ll << 18) ? kScaleGuessed
+                                                                                   : kScaleFound;
     p.values = values;
     p.valuesLd = valuesLd;
     p.blocks = mxBlocks(out.format, out.cols);

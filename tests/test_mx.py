@@ -203,6 +203,69 @@ def test_large_matrices(dev, fmt, dtype, rows, cols):
         assert torch.equal(back[:, :cols].cpu().nan_to_num(nan=12345.0), want) and (back[:, cols:] == 7.0).all()
 
 
+def read_once_input(kind, dtype, rows, cols):
+    """More than 128 MB, of which a part may say little about the rest."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(rows, cols, device="cuda", generator=g)
+    if kind == "outlier":
+        x[1, cols // 2] = 3000.0
+    elif kind == "few rows":
+        keep = x[[1, 778, rows - 1]] * 2.0 ** -5
+        x.zero_()
+        x[[1, 778, rows - 1]] = keep
+    elif kind == "steep":
+        x *= 2.0 ** torch.randint(-14, 9, (rows, 1), device="cuda", generator=g)
+        x[:, :cols // 3] *= 2.0 ** -9
+        x[torch.rand(rows, device="cuda", generator=g) < 0.3] = 0.0
+        x[5, 0], x[6, cols - 1], x[7, cols // 2] = float("nan"), float("inf"), -float("inf")
+        x[9] = float("nan")
+    elif kind == "tiny":
+        x *= 2.0 ** -141
+    elif kind == "huge":
+        x[3] *= 2.0 ** 110
+        x[rows - 2] *= 2.0 ** 120
+    elif kind == "zero":
+        x.zero_()
+    return x.to(TYPES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype,rows,cols,layout", [
+    ("normal", A.F16, 16384, 4096, A.MX_SCALES_TILED), ("normal", A.F16, 16400, 4099, A.MX_SCALES_TILED),
+    ("outlier", A.F16, 16400, 4099, A.MX_SCALES_ROWS), ("outlier", A.BF16, 16403, 4096, A.MX_SCALES_TILED),
+    ("few rows", A.F32, 8200, 4096, A.MX_SCALES_TILED), ("few rows", A.F16, 8400000, 5, A.MX_SCALES_ROWS),
+    ("steep", A.F32, 8199, 4111, A.MX_SCALES_TILED), ("steep", A.BF16, 1680000, 40, A.MX_SCALES_TILED),
+    ("steep", A.F16, 600, 120000, A.MX_SCALES_ROWS), ("tiny", A.F32, 8200, 4096, A.MX_SCALES_ROWS),
+    ("huge", A.F32, 540, 65535, A.MX_SCALES_TILED), ("zero", A.F32, 8200, 4096, A.MX_SCALES_TILED)])
+@pytest.mark.parametrize("offset", [0, 5])
+def test_matrices_that_are_read_once(dev, kind, dtype, rows, cols, layout, offset):
+    """Their factor is guessed and put right: the bytes are those of the right factor given from the start."""
+    x = read_once_input(kind, dtype, rows, cols)
+    top = float(x.float().abs().nan_to_num(nan=0.0, posinf=0.0).max())
+    t = O.tensor_scale_of(top)
+    runs = []
+    for given in (None, t):
+        h = Held(A.NVFP4, rows, cols, layout, t=given)
+        if layout == A.MX_SCALES_ROWS:  # which may start anywhere
+            h.m = mx.MxMatrix(A.NVFP4, rows, cols, h.codes.data_ptr(), h.scales.data_ptr() + offset, h.tensor.data_ptr(), ld=h.ld, layout=layout)
+        values = torch.full((rows, cols), 7.0, dtype=x.dtype, device="cuda")
+        dev.mx_quantize(x.data_ptr(), dtype, cols, h.m, values=values.data_ptr(), values_ld=cols, tensor_scale_given=given is not None)
+        runs.append((h, values))
+        if given is None:
+            assert h.tensor.tolist() == [float(t), top]
+    (found, values), (right, right_values) = runs
+    assert torch.equal(found.scales, right.scales) and torch.equal(found.codes, right.codes)
+    bits = torch.int32 if dtype == A.F32 else torch.int16
+    assert torch.equal(values.view(bits), right_values.view(bits))
+    some = torch.randint(0, rows, (40,)).unique().tolist() + [1, 5, rows - 1]
+    q = O.quantize(x[some].cpu().double().numpy(), A.NVFP4, t=t)
+    codes = found.codes[:rows * found.ld].view(rows, found.ld)[some].cpu().numpy()
+    np.testing.assert_array_equal(codes[:, :found.pitch], O.pack(q["codes"]))
+    if layout == A.MX_SCALES_ROWS:
+        scales = found.scales[offset:offset + found.nscale].view(rows, -1)[some].cpu().numpy()
+        np.testing.assert_array_equal(scales, q["scales"])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", [1.0, 0.37, 2.0 ** -9, 3e-30, 1e30])
 @pytest.mark.parametrize("dtype", list(TYPES))
