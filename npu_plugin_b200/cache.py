@@ -16,6 +16,9 @@ values; the bytes kept here are the converted ones, so a prefix is reused only w
 storage element type equals its logical one, it is not a splat and not sub-byte -- and any other request is
 folded from the base content.  Results are therefore always those of a direct fold.
 
+What a fold writes beside its bytes (the scales of a QuantizeMx) is kept with the content, in arrays of its own, and copied
+to the arrays of whoever is answered from the cache.  A key holds the objects that it tells apart by identity.
+
 A "context" (the reference's MLIRContext) is any hashable object the caller compiles under; here the backend.
 """
 import queue
@@ -239,6 +242,16 @@ def prefix_is_reusable(attr):
 
 
 # --------------------------------------------------------------------------- background folding
+def _fold_with_own_sides(backend, base_type, data, is_splat, transforms, first):
+    """fold_resident, with the arrays that it writes kept by the content: nobody's own are touched before fold() asks.
+    first: position in the attribute's list of the first of `transforms`."""
+    own = [t.withOwnSides() if t.kind in t.WRITES_SIDES else t for t in transforms]
+    content = backend.fold_resident(base_type, data, is_splat, own)
+    content.sides = [(first + k, name, getattr(t, name)) for k, t in enumerate(own) if t.kind in t.WRITES_SIDES
+                     for name in ("side0", "side1") if getattr(t, name) is not None]
+    return content
+
+
 def tryFoldingPartially(cache, request, newTransformation):
     if newTransformation is None:
         return False
@@ -255,7 +268,9 @@ def tryFoldingPartially(cache, request, newTransformation):
         return False
     cache.setRequestState(request, FoldingRequestState.PENDING)
     # the remaining transformations are folded over the cached bytes, which stay where they are (device memory)
-    content = request._backend.fold_resident(partial.type_as_base(), partial, False, last)
+    first = len(partial_attr.getTransformations())
+    content = _fold_with_own_sides(request._backend, partial.type_as_base(), partial, False, last, first)
+    content.sides = partial.sides + content.sides
     cache.addContent(request, content)
     cache.removeContent(partial_attr)
     cache.setRequestState(request, FoldingRequestState.COMPLETED)
@@ -280,8 +295,8 @@ def _folding_thread(ctx):
             if tryFoldingPartially(cache, request, req.newTransformation):
                 continue
             cache.setRequestState(request, FoldingRequestState.PENDING)
-            content = request._backend.fold_resident(request._baseType, request._base, request._isSplat,
-                                                     request.getTransformations())
+            content = _fold_with_own_sides(request._backend, request._baseType, request._base, request._isSplat,
+                                           request.getTransformations(), 0)
             cache.addContent(request, content)
         except Exception as e:  # a request that cannot be folded (the foreground fold raises the same error)
             cache.addContent(request, FailedContent(e))

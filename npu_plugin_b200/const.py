@@ -9,6 +9,7 @@ libb200const.so on the GPU; this module only marshals descriptors.
 A `backend` object supplies infer_type / insert_position / fold / ...; the default is the CUDA
 library.  Tests pass the CPU oracle's backend to run the same chain on both sides.
 """
+import copy
 import ctypes as C
 
 import numpy as np
@@ -216,24 +217,66 @@ _NAMES = {A.X_CONVERT_ELEM_TYPE: "ConvertElemType", A.X_QUANT_CAST: "QuantCast",
           A.X_QUANTIZE_SYNTH: "QuantizeSynth", A.X_QUANTIZE_MX: "QuantizeMx", A.X_DEQUANTIZE_MX: "DequantizeMx"}
 
 
+class _Same:
+    """An object as part of a key: equal to itself alone, and alive as long as the key is, so that no later object at its
+    address can be taken for it."""
+
+    __slots__ = ("of",)
+
+    def __init__(self, of):
+        self.of = of
+
+    def __eq__(self, o):
+        return isinstance(o, _Same) and self.of is o.of
+
+    def __hash__(self):
+        return id(self.of)
+
+
 class Transform:
-    """One Const::TransformAttrInterface instance."""
+    """One Const::TransformAttrInterface instance.  side0 / side1: arrays that the fold writes, or (DequantizeMx) reads --
+    those are copied here, since they are part of the transformation's value."""
+
+    WRITES_SIDES = (A.X_QUANTIZE_MX,)
 
     def __init__(self, kind, a=(), b=(), f=0.0, i0=0, i1=0, elem=None, aux=None, side0=None, side1=None):
         self.kind, self.a, self.b, self.f, self.i0, self.i1 = kind, tuple(a), tuple(b), float(f), int(i0), int(i1)
         self.elem, self.aux, self.side0, self.side1 = elem, (None if aux is None else [int(v) for v in aux]), side0, side1
+        self._read = ()
+        if kind == A.X_DEQUANTIZE_MX:
+            # as bytes: nobody can change them, and their hash is computed once
+            self._read = tuple(s.tobytes() if isinstance(s, np.ndarray) else s for s in (side0, side1))
+            self.side0, self.side1 = (np.frombuffer(b, s.dtype).reshape(s.shape) if isinstance(s, np.ndarray) else s
+                                      for b, s in zip(self._read, (side0, side1)))
 
     def getTransformationName(self):
         return _NAMES[self.kind]
 
-    def key(self):
-        """Value identity of the transformation (MLIR attributes are uniqued by value)."""
+    def valueKey(self):
+        """What the folded bytes depend on.  Of arrays that the fold writes only their sizes: which bytes land there is
+        the same for all that are asked for."""
         e = self.elem
         ek = (e.kind, e.storage, e.expressed, tuple(e.scales), tuple(e.zps), e.axis, e.qmin, e.qmax) if isinstance(e, Quant) else e
-        # the scales that QuantizeMx writes and DequantizeMx reads belong to the transformation, as a base content does
-        # to its attribute: two with scales of their own are not one
-        mine = (id(self.side0), id(self.side1)) if self.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX) else ()
-        return (self.kind, self.a, self.b, self.f, self.i0, self.i1, ek, None if self.aux is None else tuple(self.aux)) + mine
+        sides = self._read
+        if self.kind in self.WRITES_SIDES:
+            sides = tuple(s.nbytes if isinstance(s, np.ndarray) else s for s in (self.side0, self.side1))
+        return (self.kind, self.a, self.b, self.f, self.i0, self.i1, ek, None if self.aux is None else tuple(self.aux)) + sides
+
+    def key(self):
+        """Identity of the transformation (MLIR attributes are uniqued by value): two QuantizeMx with arrays of their own
+        for the scales are not one."""
+        mine = (_Same(self.side0), _Same(self.side1)) if self.kind == A.X_QUANTIZE_MX else ()
+        return self.valueKey() + mine
+
+    def usesPointers(self):
+        """The caller's memory stands in for a side array: what lies there is not known to whoever keeps the result."""
+        return any(s is not None and not isinstance(s, np.ndarray) for s in (self.side0, self.side1))
+
+    def withOwnSides(self):
+        """The same transformation writing into new arrays."""
+        out = copy.copy(self)
+        out.side0, out.side1 = (None if s is None else np.zeros_like(s) for s in (self.side0, self.side1))
+        return out
 
     def __eq__(self, o):
         return isinstance(o, Transform) and self.key() == o.key()
@@ -354,6 +397,7 @@ class ResidentContent:
 
     def __init__(self, backend, ndtype, buf, nbytes, written):
         self.backend, self.type, self.buf, self.nbytes, self.written = backend, ndtype, buf, int(nbytes), int(written)
+        self.sides = []  # (position in the list, "side0" or "side1", array) of what the fold wrote beside the bytes
         self._released = False
 
     def type_as_base(self):
@@ -752,14 +796,18 @@ class ContentAttr:
         # with background folding enabled for this context, the new attribute is folded ahead of time (content.cpp:320-328)
         from .cache import ConstantFoldingCacheManager, FoldingRequest
         mgr = ConstantFoldingCacheManager.getInstance()
-        if mgr.contains(self._backend):
+        if mgr.contains(self._backend) and out.isCacheable():
             mgr.get(self._backend).enqueueRequest(FoldingRequest(out, t))
         return out
 
     def key(self):
         """Value identity: the base content object, its type and splat flag, and the transformation list."""
         bt = self._baseType
-        return (id(self._base), bt.shape, bt.dtype, tuple(bt.order), self._isSplat, tuple(t.key() for t in self._transforms))
+        return (_Same(self._base), bt.shape, bt.dtype, tuple(bt.order), self._isSplat,
+                tuple(t.valueKey() for t in self._transforms))
+
+    def isCacheable(self):
+        return not any(t.usesPointers() for t in self._transforms)
 
     # -- ContentAttr::stripTransformationsFrom / getLastTransformationsFrom (content.cpp:342-369): the rightmost
     #    occurrence of the transformation splits the list
@@ -863,7 +911,7 @@ class ContentAttr:
 
     def dequantizeMx(self, fmt, elem, scales=None, tensorScale=None):
         """What 4-bit floats stand for, as `elem` (A.F16, A.BF16 or A.F32).  scales (uint8 [rows, blocks]) and, for nvfp4,
-        tensorScale (float32, the first counts): arrays, or None right behind a quantizeMx."""
+        tensorScale (float32, the first counts): arrays, which are copied, or None right behind a quantizeMx."""
         s0 = None if scales is None else np.ascontiguousarray(scales, np.uint8)
         s1 = None if tensorScale is None else np.ascontiguousarray(tensorScale, np.float32).reshape(-1)
         if s0 is not None:
@@ -908,11 +956,13 @@ class ContentAttr:
         if not bypassCache:
             from .cache import ConstantFoldingCacheManager, FailedContent
             mgr = ConstantFoldingCacheManager.getInstance()
-            if mgr.contains(self._backend):
+            if mgr.contains(self._backend) and self.isCacheable():
                 hit = mgr.get(self._backend).getContent(self)
                 if isinstance(hit, FailedContent):
                     raise hit.error
                 if hit is not None:
+                    for at, name, array in hit.sides:  # what a fold of this attribute would have written
+                        getattr(self._transforms[at], name).view(np.uint8).reshape(-1)[:] = array.view(np.uint8).reshape(-1)
                     return hit.to_content()
         return self._backend.fold(self._baseType, self._base, self._isSplat, self._transforms)
 

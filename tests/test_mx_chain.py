@@ -1,5 +1,8 @@
 """Block-scaled 4-bit floats as transformations of a constant: QuantizeMx and DequantizeMx in chains, in batched folds,
 through the constant-folding pass, and the chain builder that decides whether a layer's weights may be held so."""
+import gc
+import time
+
 import numpy as np
 import pytest
 
@@ -7,7 +10,10 @@ import mx_oracle as O
 from npu_plugin_b200 import _cabi as A
 from npu_plugin_b200 import chains
 from npu_plugin_b200.blob import ConstantDecl, ShardFolder
-from npu_plugin_b200.const import ConstError, ContentAttr, DeclareOp, DimsOrder, NDType, Transform, Unsupported, constant_folding_pass
+from npu_plugin_b200.cache import (ConstantFoldingCacheManager, initBackgroundConstantFoldingThreads,
+                                   stopBackgroundConstantFoldingThreads)
+from npu_plugin_b200.const import (ConstError, Content, ContentAttr, DeclareOp, DimsOrder, NDType, ResidentContent, Transform,
+                                   Unsupported, constant_folding_pass)
 from test_abi_and_host import HostOnly
 
 FORMATS = [A.MXFP4, A.NVFP4]
@@ -67,6 +73,136 @@ def test_two_transformations_with_their_own_scales_are_not_one():
     s = np.zeros((8, 2), np.uint8)
     assert Q(A.MXFP4, side0=s) == Q(A.MXFP4, side0=s)
     assert Q(A.MXFP4, side0=s) != Q(A.MXFP4, side0=s.copy())
+
+
+# --------------------------------------------------------------------------- background folding
+class FakeDevice(HostOnly):
+    """Folds lists of one QuantizeMx and one DequantizeMx with the oracle, into host memory."""
+
+    def __init__(self):
+        super().__init__()
+        self.folds = 0
+
+    def _run(self, base_type, data, transforms):
+        self.folds += 1
+        q = None
+        for t in transforms:
+            rows, cols = base_type.shape
+            if t.kind == A.X_QUANTIZE_MX:
+                q = O.quantize(data.astype(np.float64), t.i0, t=t.f or None)
+                t.side0[:] = q["scales"]
+                if t.i0 == A.NVFP4:
+                    t.side1[:] = q["t"], q["top"]
+                out = O.pack(q["codes"]).reshape(-1)
+            else:
+                packed = data.reshape(rows, -1) if q is None else O.pack(q["codes"])
+                codes = np.stack([packed & 15, packed >> 4], 2).reshape(rows, -1)[:, :cols]
+                scales = q["scales"] if t.side0 is None else t.side0.reshape(rows, -1)
+                factor = q["t"] if t.side0 is None else None if t.side1 is None else t.side1[0]
+                out = O.values_of(codes, scales, t.i0, factor).astype(np.float32).reshape(-1)
+        return out.view(np.uint8)
+
+    def fold(self, base_type, data, is_splat, transforms):
+        out = self._run(base_type, data, transforms)
+        return Content(self.infer_type(base_type, transforms), out, out.size)
+
+    def fold_resident(self, base_type, data, is_splat, transforms):
+        out = self._run(base_type, data, transforms)
+        return ResidentContent(self, self.infer_type(base_type, transforms), out, out.size, out.size)
+
+    def resident_to_host(self, rc):
+        return rc.buf
+
+    def free_resident(self, rc):
+        rc.buf = None
+
+
+@pytest.fixture(params=["fake", pytest.param("b200", marks=pytest.mark.gpu)])
+def folding_ahead(request):
+    """A context whose attributes are folded by two threads as they are built."""
+    if request.param == "fake":
+        ctx = FakeDevice()
+    else:
+        from npu_plugin_b200.const import CudaBackend
+        ctx = CudaBackend(0)
+    threads = initBackgroundConstantFoldingThreads(ctx, 2)
+    yield ctx
+    stopBackgroundConstantFoldingThreads(ctx, threads)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_each_attribute_receives_its_scales_from_the_cache(folding_ahead, fmt):
+    """Attributes of one base that are built, folded and dropped: an address that comes back is another array."""
+    w = np.random.default_rng(11).normal(0, 1, (6, 64)).astype(np.float32)
+    want = O.quantize(w.astype(np.float64), fmt)
+    base = ContentAttr.get(w, backend=folding_ahead)
+    for _ in range(20):
+        q = base.quantizeMx(fmt)
+        np.testing.assert_array_equal(q.fold().copyTo(), O.pack(want["codes"]).reshape(-1))
+        np.testing.assert_array_equal(q.mxScales, want["scales"])
+        if fmt == A.NVFP4:
+            assert q.mxTensorScale.tolist() == [want["t"], want["top"]]
+        back = q.dequantizeMx(fmt, A.F32)
+        q.mxScales[:] = 0
+        np.testing.assert_array_equal(back.fold().getValues().reshape(w.shape), want["values"].astype(np.float32))
+        np.testing.assert_array_equal(q.mxScales, want["scales"])  # those of one transformation: written again
+        del q, back
+        gc.collect()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_each_attribute_is_read_with_its_own_scales(folding_ahead, fmt):
+    rng = np.random.default_rng(12)
+    codes = rng.integers(0, 16, (6, 64)).astype(np.uint8)
+    base = ContentAttr.get(O.pack(codes).reshape(-1), NDType((6, 64), A.F4E2M1), is_splat=False, backend=folding_ahead)
+    blocks = (6, 64 // O.BLOCK[fmt])
+    scales, factor = np.zeros(blocks, np.uint8), np.zeros(2, np.float32)
+    for i in range(20):
+        if i % 2:  # the same arrays with other numbers in them, or others that may come to lie where the last ones did
+            scales, factor = np.empty(blocks, np.uint8), np.empty(2, np.float32)
+        scales[:], factor[0] = rng.integers(40, 80, blocks), rng.uniform(0.5, 2.0)
+        want = O.values_of(codes, scales, fmt, factor[0])
+        a = base.dequantizeMx(fmt, A.F32, scales, factor if fmt == A.NVFP4 else None)
+        scales[:], factor[0] = 0, 0  # what was given counts
+        # scale * factor is rounded to 32 bits, code times that again: half a unit of 2^-23 each, and their product
+        np.testing.assert_allclose(a.fold().getValues().reshape(6, 64).astype(np.float64), want, rtol=2 * 2.0 ** -24 * 1.001, atol=0)
+        del a
+        gc.collect()
+
+
+def test_bases_at_one_address_are_not_one(folding_ahead):
+    for i in range(20):
+        q = ContentAttr.get(np.full((1, 32), i + 1.0, np.float32), is_splat=False, backend=folding_ahead).quantizeMx(A.MXFP4)
+        q.fold()
+        np.testing.assert_array_equal(q.mxScales, O.quantize(np.full((1, 32), i + 1.0), A.MXFP4)["scales"])
+        del q
+        gc.collect()
+
+
+def test_one_fold_answers_all_that_ask_for_the_same():
+    ctx = FakeDevice()
+    w = np.random.default_rng(13).normal(0, 1, (6, 64)).astype(np.float32)
+    base = ContentAttr.get(w, backend=ctx)
+    threads = initBackgroundConstantFoldingThreads(ctx, 1)
+    attrs = [base.quantizeMx(A.MXFP4) for _ in range(5)]
+    while not ConstantFoldingCacheManager.getInstance().get(ctx)._requests.empty():
+        time.sleep(0.01)
+    for a in attrs:
+        a.fold()
+        assert (a.mxScales == attrs[0].mxScales).all() and (a.mxScales != 0).all()
+    assert ctx.folds == 1 and attrs[0] is not attrs[1] and attrs[0].mxScales is not attrs[1].mxScales
+    stopBackgroundConstantFoldingThreads(ctx, threads)
+
+
+def test_the_callers_memory_is_never_read_or_written_ahead():
+    """Side arrays given as addresses: nobody but the caller knows what lies there, and when."""
+    ctx = FakeDevice()
+    threads = initBackgroundConstantFoldingThreads(ctx, 1)
+    base = ContentAttr.get(np.zeros((2, 32), np.float32), is_splat=False, backend=ctx)
+    a = base.addTransformation(Q(A.MXFP4, side0=0x1000))
+    b = a.addTransformation(D(A.MXFP4))
+    stopBackgroundConstantFoldingThreads(ctx, threads)
+    assert ctx.folds == 0 and not a.isCacheable() and not b.isCacheable() and base.quantizeMx(A.MXFP4).isCacheable()
 
 
 # --------------------------------------------------------------------------- on the device
