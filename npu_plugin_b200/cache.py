@@ -16,7 +16,7 @@ values; the bytes kept here are the converted ones, so a prefix is reused only w
 storage element type equals its logical one, it is not a splat and not sub-byte -- and any other request is
 folded from the base content.  Results are therefore always those of a direct fold.
 
-What a fold writes beside its bytes (the scales of a QuantizeMx) is kept with the content, in arrays of its own, and copied
+What a fold writes beside its bytes (the scales of a QuantizeMx or QuantizeSynth) is kept with the content, in arrays of its own, and copied
 to the arrays of whoever is answered from the cache.  A key holds the objects that it tells apart by identity.
 
 A "context" (the reference's MLIRContext) is any hashable object the caller compiles under; here the backend.

@@ -237,7 +237,7 @@ class Transform:
     """One Const::TransformAttrInterface instance.  side0 / side1: arrays that the fold writes, or (DequantizeMx) reads --
     those are copied here, since they are part of the transformation's value."""
 
-    WRITES_SIDES = (A.X_QUANTIZE_MX,)
+    WRITES_SIDES = (A.X_QUANTIZE_SYNTH, A.X_QUANTIZE_MX)
 
     def __init__(self, kind, a=(), b=(), f=0.0, i0=0, i1=0, elem=None, aux=None, side0=None, side1=None):
         self.kind, self.a, self.b, self.f, self.i0, self.i1 = kind, tuple(a), tuple(b), float(f), int(i0), int(i1)
@@ -252,21 +252,20 @@ class Transform:
     def getTransformationName(self):
         return _NAMES[self.kind]
 
-    def valueKey(self):
-        """What the folded bytes depend on.  Of arrays that the fold writes only their sizes: which bytes land there is
-        the same for all that are asked for."""
-        e = self.elem
-        ek = (e.kind, e.storage, e.expressed, tuple(e.scales), tuple(e.zps), e.axis, e.qmin, e.qmax) if isinstance(e, Quant) else e
-        sides = self._read
-        if self.kind in self.WRITES_SIDES:
-            sides = tuple(s.nbytes if isinstance(s, np.ndarray) else s for s in (self.side0, self.side1))
-        return (self.kind, self.a, self.b, self.f, self.i0, self.i1, ek, None if self.aux is None else tuple(self.aux)) + sides
-
     def key(self):
         """Identity of the transformation (MLIR attributes are uniqued by value): two QuantizeMx with arrays of their own
         for the scales are not one."""
-        mine = (_Same(self.side0), _Same(self.side1)) if self.kind == A.X_QUANTIZE_MX else ()
-        return self.valueKey() + mine
+        e = self.elem
+        ek = (e.kind, e.storage, e.expressed, tuple(e.scales), tuple(e.zps), e.axis, e.qmin, e.qmax) if isinstance(e, Quant) else e
+        mine = (_Same(self.side0), _Same(self.side1)) if self.kind == A.X_QUANTIZE_MX else self._read
+        return (self.kind, self.a, self.b, self.f, self.i0, self.i1, ek, None if self.aux is None else tuple(self.aux)) + mine
+
+    def valueKey(self):
+        """What the folded bytes depend on.  Of arrays that the fold writes only their sizes: which bytes land there is
+        the same for all that are asked for."""
+        if self.kind not in self.WRITES_SIDES:
+            return self.key()
+        return self.key()[:8] + tuple(s.nbytes if isinstance(s, np.ndarray) else s for s in (self.side0, self.side1))
 
     def usesPointers(self):
         """The caller's memory stands in for a side array: what lies there is not known to whoever keeps the result."""
@@ -488,8 +487,8 @@ class CudaBackend:
             for x, t in zip(ch, transforms):
                 for name in ("side0", "side1"):
                     host = getattr(t, name)
-                    if t.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX) and isinstance(host, np.ndarray):
-                        sides.append((self.dev_alloc(host.nbytes), host, t.kind == A.X_QUANTIZE_MX))
+                    if isinstance(host, np.ndarray):
+                        sides.append((self.dev_alloc(host.nbytes), host, t.kind in t.WRITES_SIDES))
                         self.upload(sides[-1][0], host)
                         setattr(x, name, sides[-1][0])
             self.fill_zero(out, cap)

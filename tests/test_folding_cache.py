@@ -113,6 +113,73 @@ def test_prefix_with_pending_conversion_or_splat_is_not_reused(backend):
     assert stats["partial folds"] == 0
 
 
+@pytest.mark.parametrize("scheme,store", [(A.QSYNTH_SYM_I8, A.SI8), (A.QSYNTH_ASYM_U4, A.UI8)])
+def test_scales_of_a_quantiser_that_was_folded_ahead(backend, scheme, store):
+    """Every attribute receives its scales and zero points, whoever folded it; also through a partial fold."""
+    ctx = new_context(backend)
+    threads = initBackgroundConstantFoldingThreads(ctx, 2)
+    w = np.random.default_rng(9).normal(0, 1, (8, 16, 3, 3)).astype(np.float32)
+    a = ContentAttr.get(w, backend=ctx)
+    for _ in range(6):
+        q = a.quantizeSynth(scheme)
+        chain = q.convertElemType(store).reorder(DimsOrder.NHWC)
+        got = chain.fold().copyTo()
+        scales, zps = chain.sideScales.copy(), chain.sideZeroPoints.copy()
+        chain.sideScales[:], chain.sideZeroPoints[:] = 0, 0
+        assert np.array_equal(got, chain.fold(bypassCache=True).copyTo())
+        assert np.array_equal(scales, chain.sideScales) and np.array_equal(zps, chain.sideZeroPoints) and (scales != 0).all()
+    stopBackgroundConstantFoldingThreads(ctx, threads)
+
+
+def test_a_resident_fold_gives_the_device_no_host_address():
+    """Its side arrays lie on the device while it runs, and are copied back."""
+    import ctypes as C
+    from npu_plugin_b200 import const as K
+
+    class Recorder(K.CudaBackend):
+        """The marshalling of the CUDA backend over memory that is only counted."""
+        ctx = None
+
+        def __init__(self):
+            self.lib, self.at, self.blocks = self, 1 << 40, {}
+            self.real = A.load()
+            self.b200c_infer_type, self.b200c_last_error = self.real.b200c_infer_type, self.real.b200c_last_error
+
+        def dev_alloc(self, nbytes):
+            self.at += 1 << 20
+            self.blocks[self.at] = nbytes
+            return self.at
+
+        def dev_free(self, ptr):
+            del self.blocks[ptr]
+
+        def upload(self, ptr, array):
+            assert array.nbytes == self.blocks[ptr]
+
+        def download(self, ptr, nbytes):
+            return np.full(nbytes, 3, np.uint8)
+
+        def fill_zero(self, ptr, nbytes):
+            pass
+
+        def b200c_fold(self, ctx, bt, src, n, splat, on_dev, chain, count, out, cap, out_on_dev, nb, ot, flags):
+            assert out_on_dev
+            self.given = [p for k in range(count) for p in (chain[k].side0, chain[k].side1) if p]
+            assert all(p in self.blocks for p in self.given)
+            bare = (A.b200c_xform * count)(*[chain[k] for k in range(count)])
+            return self.real.b200c_infer_type(bt, bare, count, ot)
+
+    r = Recorder()
+    s = [np.zeros(4, np.float32), np.zeros(4, np.int32), np.zeros((4, 4), np.uint8), np.zeros(2, np.float32)]
+    x = np.ones((4, 64), np.float32)
+    for t, sides in ((K.Transform(A.X_QUANTIZE_SYNTH, i0=A.QSYNTH_SYM_I8, side0=s[0], side1=s[1]), s[:2]),
+                     (K.Transform(A.X_QUANTIZE_MX, i0=A.NVFP4, side0=s[2], side1=s[3]), s[2:])):
+        content = r.fold_resident(NDType((4, 64), A.F32), x, False, [t])
+        assert len(r.given) == 2 and list(r.blocks) == [content.buf]
+        assert all((a.view(np.uint8) == 3).all() for a in sides)
+        r.dev_free(content.buf)
+
+
 def test_failing_request_raises_in_the_foreground(backend):
     from npu_plugin_b200.const import ConstError
     ctx = new_context(backend)
