@@ -266,11 +266,16 @@ def tryFoldingPartially(cache, request, newTransformation):
         return False
     if not prefix_is_reusable(partial_attr):
         return False
-    cache.setRequestState(request, FoldingRequestState.PENDING)
-    # the remaining transformations are folded over the cached bytes, which stay where they are (device memory)
-    first = len(partial_attr.getTransformations())
-    content = _fold_with_own_sides(request._backend, partial.type_as_base(), partial, False, last, first)
-    content.sides = partial.sides + content.sides
+    if not partial.use():  # failed, or dropped by another thread whose request starts with it too
+        return False
+    try:
+        cache.setRequestState(request, FoldingRequestState.PENDING)
+        # the remaining transformations are folded over the cached bytes, which stay where they are (device memory)
+        first = len(partial_attr.getTransformations())
+        content = _fold_with_own_sides(request._backend, partial.type_as_base(), partial, False, last, first)
+        content.sides = partial.sides + content.sides
+    finally:
+        partial.done()
     cache.addContent(request, content)
     cache.removeContent(partial_attr)
     cache.setRequestState(request, FoldingRequestState.COMPLETED)
@@ -309,6 +314,9 @@ class FailedContent:
 
     def __init__(self, error):
         self.error = error
+
+    def use(self):
+        return False
 
     def release(self):
         pass

@@ -11,6 +11,7 @@ library.  Tests pass the CPU oracle's backend to run the same chain on both side
 """
 import copy
 import ctypes as C
+import threading
 
 import numpy as np
 
@@ -398,6 +399,22 @@ class ResidentContent:
         self.backend, self.type, self.buf, self.nbytes, self.written = backend, ndtype, buf, int(nbytes), int(written)
         self.sides = []  # (position in the list, "side0" or "side1", array) of what the fold wrote beside the bytes
         self._released = False
+        self._users, self._lock = 1, threading.Lock()
+
+    def use(self):
+        """Keeps the buffer until done(), whoever releases it in between; False if it is gone already."""
+        with self._lock:
+            if self._users == 0:
+                return False
+            self._users += 1
+            return True
+
+    def done(self):
+        with self._lock:
+            self._users -= 1
+            last = self._users == 0
+        if last:
+            self.backend.free_resident(self)
 
     def type_as_base(self):
         """The type a base content of these bytes has: shape, storage element type and order (quantisation
@@ -411,7 +428,7 @@ class ResidentContent:
     def release(self):
         if not self._released:
             self._released = True
-            self.backend.free_resident(self)
+            self.done()
 
 
 # --------------------------------------------------------------------------- backend (CUDA library)
@@ -959,10 +976,13 @@ class ContentAttr:
                 hit = mgr.get(self._backend).getContent(self)
                 if isinstance(hit, FailedContent):
                     raise hit.error
-                if hit is not None:
-                    for at, name, array in hit.sides:  # what a fold of this attribute would have written
-                        getattr(self._transforms[at], name).view(np.uint8).reshape(-1)[:] = array.view(np.uint8).reshape(-1)
-                    return hit.to_content()
+                if hit is not None and hit.use():
+                    try:
+                        for at, name, array in hit.sides:  # what a fold of this attribute would have written
+                            getattr(self._transforms[at], name).view(np.uint8).reshape(-1)[:] = array.view(np.uint8).reshape(-1)
+                        return hit.to_content()
+                    finally:
+                        hit.done()
         return self._backend.fold(self._baseType, self._base, self._isSplat, self._transforms)
 
     def countNonSparseElementsPerOC(self):

@@ -180,6 +180,56 @@ def test_a_resident_fold_gives_the_device_no_host_address():
         r.dev_free(content.buf)
 
 
+def test_a_content_stays_while_it_is_read(oracle):
+    """Dropped by another thread in the middle: by a fold on top of it, or a reader that brings it to the host."""
+    from oracle_backend import OracleBackend
+    from npu_plugin_b200.cache import FoldingRequest, tryFoldingPartially
+    from npu_plugin_b200.const import ResidentContent
+
+    class Interrupted(OracleBackend):
+        """Somebody drops the prefix whenever it is about to be read."""
+
+        def fold_resident(self, base_type, data, is_splat, transforms):
+            if isinstance(data, ResidentContent):
+                self.cache.removeContent(self.prefix)
+            return super().fold_resident(base_type, data, is_splat, transforms)
+
+        def resident_to_host(self, rc):
+            self.cache.removeContent(self.prefix)
+            return super().resident_to_host(rc).copy()
+
+    ctx = Interrupted()
+    threads = initBackgroundConstantFoldingThreads(ctx, 0)
+    cache = ctx.cache = ConstantFoldingCacheManager.getInstance().get(ctx)
+    w = np.arange(8, dtype=np.float32)
+    ctx.prefix = ContentAttr.get(w, backend=ctx).add(1.0)
+
+    def put():
+        content = ctx.fold_resident(ctx.prefix._baseType, w, False, ctx.prefix.getTransformations())
+        cache.addContent(ctx.prefix, content)
+        cache.setRequestState(ctx.prefix, "COMPLETED")
+        return content
+
+    content = put()
+    both = ctx.prefix.rescale(2.0)
+    assert tryFoldingPartially(cache, both, both.getTransformations()[-1])
+    assert np.array_equal(both.fold().copyTo().view(np.float32), (w + 1) * 2) and content.buf is None
+    content = put()
+    assert np.array_equal(ctx.prefix.fold().copyTo().view(np.float32), w + 1) and content.buf is None
+    assert not content.use()  # gone: a request on top of it starts from the base
+    stopBackgroundConstantFoldingThreads(ctx, threads)
+
+
+def test_an_attribute_on_top_of_a_failing_one_fails_alike(backend):
+    from npu_plugin_b200.const import ConstError
+    ctx = new_context(backend)
+    threads = initBackgroundConstantFoldingThreads(ctx, 1)
+    bad = ContentAttr.get(np.array([300.0, 1.0], np.float32), backend=ctx).convertElemType(A.UI8)
+    with pytest.raises(ConstError):
+        bad.reshape((1, 2)).fold()
+    stopBackgroundConstantFoldingThreads(ctx, threads)
+
+
 def test_failing_request_raises_in_the_foreground(backend):
     from npu_plugin_b200.const import ConstError
     ctx = new_context(backend)
