@@ -318,6 +318,46 @@ __device__ __forceinline__ float toOut<float>(float v) {
     return v;
 }
 
+// What a sum is multiplied with, one factor after the other.  Where the product of the tensor scales is a normal number
+// it is the first, and the second is 1.  Otherwise that product would lose what the result still has -- two matrices
+// of size 2^-64 have scales around 2^-75, whose product 32 bits do not hold -- or be an infinity that makes NaN of a sum of
+// zeros.  Sums are 0 or lie within 2^-20 .. 2^54 (codes of 0.5 with scales of 2^-9 on both sides; 36 * 448^2 for each
+// of 2^31 elements), so the exponent is shared out evenly: a product with the first factor is below the normal numbers
+// only where the result is 0 anyway, and above the largest only where the result is, too.
+struct Factors {
+    float first, second;
+};
+__device__ __noinline__ Factors farFactors(float tp, float tq) {
+    int ep, eq;
+    const float m = frexpf(tp, &ep) * frexpf(tq, &eq);
+    // beyond these the result is 0 or infinity whatever the sum
+    const int e = min(max(ep + eq, -212), 200);
+    return Factors{ldexpf(m, e / 2), ldexpf(1.f, e - e / 2)};
+}
+__device__ __forceinline__ Factors factorsOf(const MxMatmulParams& g) {
+    if (!g.tensorP) return Factors{1.f, 1.f};
+    const float tp = g.tensorP[0], tq = g.tensorQ[0], product = tp * tq;
+    const bool normal = fabsf(product) >= 1.17549435e-38f && fabsf(product) <= 3.402823466e38f;
+    // a scale that is 0, infinite or NaN has only the product that it has
+    if (normal || tp == 0.f || tq == 0.f || !(fabsf(tp) <= 3.402823466e38f && fabsf(tq) <= 3.402823466e38f)) return Factors{product, 1.f};
+    return farFactors(tp, tq);
+}
+
+// N sums times both factors, two at a time
+template <int N>
+__device__ __forceinline__ void scaled(const Factors& f, float* v) {
+    static_assert(N % 2 == 0, "pairs");
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        asm("{\n\t.reg .b64 v, a, b;\n\t"
+            "mov.b64 v, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\tmov.b64 b, {%3, %3};\n\t"
+            "mul.rn.f32x2 v, v, a;\n\tmul.rn.f32x2 v, v, b;\n\t"
+            "mov.b64 {%0, %1}, v;\n\t}"
+            : "+f"(v[i]), "+f"(v[i + 1])
+            : "f"(f.first), "f"(f.second));
+    }
+}
+
 // The single-CTA kernel's P is the right matrix: N accumulator columns of lane p are N rows of the product at
 // column p, and a warp's lanes store 32 neighbours at a time.
 template <class T, int N>
@@ -335,7 +375,7 @@ __device__ __forceinline__ void storeAcross(const MxMatmulParams& g, long long p
     }
 }
 template <class T, int BN>
-__device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int acc, long long p, long long q0, float alpha) {
+__device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int acc, long long p, long long q0, const Factors& f) {
     constexpr int n = BN < 32 ? BN : 32;
 #pragma unroll 1
     for (int c = 0; c < BN && q0 + c < g.rowsQ; c += n) {
@@ -345,8 +385,7 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
         } else {
             readColumns16(acc + c, v);
         }
-#pragma unroll
-        for (int i = 0; i < n; ++i) v[i] = v[i] * alpha;
+        scaled<n>(f, v);
         storeAcross<T, n>(g, p, q0 + c, v);
     }
 }
@@ -357,7 +396,7 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
 // waiting for them took longer than the product itself.
 template <class T, int BN, int MOST>
 __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0,
-                                            long long q0, float alpha) {
+                                            long long q0, const Factors& f) {
     constexpr int most = 16 / MOST;
     const int c0 = static_cast<int>(rank) * BN / g.split, c1 = (static_cast<int>(rank) + 1) * BN / g.split;
     const int row = thread % 32 * 4;
@@ -386,14 +425,17 @@ __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned in
             const long long q = q0 + c + 4 * j;
             if (c + 4 * j >= cols) break;
             alignas(16) T v[4];
+            float s[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float s = w[j][0][i];
+                s[i] = w[j][0][i];
 #pragma unroll
                 for (int r = 1; r < MOST; ++r)
-                    if (r < g.split) s = s + w[j][r][i];
-                v[i] = toOut<T>(s * alpha);
+                    if (r < g.split) s[i] = s[i] + w[j][r][i];
             }
+            scaled<4>(f, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = toOut<T>(s[i]);
             T* out = static_cast<T*>(g.out);
             if (g.wide && rows == 4) {
                 T* at = out + q * g.ld + p;
@@ -413,13 +455,13 @@ __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned in
 
 template <class T, int BN>
 __device__ __forceinline__ void join(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0, long long q0,
-                                     float alpha) {
+                                     const Factors& f) {
     if (g.split <= 2) {
-        joinColumns<T, BN, 2>(g, sums, rank, thread, p0, q0, alpha);
+        joinColumns<T, BN, 2>(g, sums, rank, thread, p0, q0, f);
     } else if (g.split <= 4) {
-        joinColumns<T, BN, 4>(g, sums, rank, thread, p0, q0, alpha);
+        joinColumns<T, BN, 4>(g, sums, rank, thread, p0, q0, f);
     } else {
-        joinColumns<T, BN, 8>(g, sums, rank, thread, p0, q0, alpha);
+        joinColumns<T, BN, 8>(g, sums, rank, thread, p0, q0, f);
     }
 }
 
@@ -532,19 +574,19 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         }
     }
     __syncwarp();
+    const Factors f = factorsOf(g);  // before the wait, which hides its loads
     const bool finished = warp < 4 && __all_sync(0xFFFFFFFFu, barWait(done, 0, stalled) && !*stalled);  // the reads are the whole warp's
-    const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
     const unsigned int mine = acc + (static_cast<unsigned int>(warp * 32) << 16);
     const int row = warp * 32 + lane;
     if (finished) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (g.split == 1) {
         if (finished) {
             if (g.outTag == T_F16) {
-                epilogue<__half, BN>(g, mine, p0 + row, q0, alpha);
+                epilogue<__half, BN>(g, mine, p0 + row, q0, f);
             } else if (g.outTag == T_BF16) {
-                epilogue<__nv_bfloat16, BN>(g, mine, p0 + row, q0, alpha);
+                epilogue<__nv_bfloat16, BN>(g, mine, p0 + row, q0, f);
             } else {
-                epilogue<float, BN>(g, mine, p0 + row, q0, alpha);
+                epilogue<float, BN>(g, mine, p0 + row, q0, f);
             }
         }
     } else {
@@ -568,11 +610,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         clusterSync();
         if (finished) {
             if (g.outTag == T_F16) {
-                join<__half, BN>(g, stage0, rank, row, p0, q0, alpha);
+                join<__half, BN>(g, stage0, rank, row, p0, q0, f);
             } else if (g.outTag == T_BF16) {
-                join<__nv_bfloat16, BN>(g, stage0, rank, row, p0, q0, alpha);
+                join<__nv_bfloat16, BN>(g, stage0, rank, row, p0, q0, f);
             } else {
-                join<float, BN>(g, stage0, rank, row, p0, q0, alpha);
+                join<float, BN>(g, stage0, rank, row, p0, q0, f);
             }
         }
         __syncwarp();
@@ -602,10 +644,11 @@ __device__ __forceinline__ void tileOf(const MxMatmulParams& g, int t, int* p, i
 // different rows at a time.
 template <class T>
 __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtensorMap* mapOut, unsigned int staging, int group, int lane,
-                                           long long row0, long long col0, const unsigned int r[32], float alpha) {
+                                           long long row0, long long col0, const unsigned int r[32], const Factors& f) {
     float v[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * alpha;
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    scaled<32>(f, v);
     constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16, bufs = 2 * 128 / rowBytes;
     const unsigned int at = staging + (group % bufs) * 32 * rowBytes;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(bufs - 1) : "memory");  // the last store from here has been read
@@ -659,7 +702,7 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
 
 template <class T>
 __device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, const CUtensorMap* mapOut, unsigned int staging, unsigned int acc, int buf,
-                                             long long row0, long long q0, float alpha, unsigned int accFree, int lane) {
+                                             long long row0, long long q0, const Factors& f, unsigned int accFree, int lane) {
     // columns 160..255 of tensor memory belong to both buffers: they are read first, and the next tile may start
     const int shared0 = buf ? 0 : 160;
     unsigned int r[3][32];
@@ -671,13 +714,13 @@ __device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, const CUte
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(accFree) : "memory");
 #pragma unroll
-    for (int i = 0; i < 3; ++i) storeGroup<T>(g, mapOut, staging, i, lane, row0, q0 + shared0 + i * 32, r[i], alpha);
+    for (int i = 0; i < 3; ++i) storeGroup<T>(g, mapOut, staging, i, lane, row0, q0 + shared0 + i * 32, r[i], f);
     const int rest = buf ? 96 : 0;
 #pragma unroll 1
     for (int i = 0; i < 5; ++i) {
         startRead(acc + rest + i * 32, r[0]);
         readsDone(r[0]);
-        storeGroup<T>(g, mapOut, staging, i + 3, lane, row0, q0 + rest + i * 32, r[0], alpha);
+        storeGroup<T>(g, mapOut, staging, i + 3, lane, row0, q0 + rest + i * 32, r[0], f);
     }
 }
 
@@ -795,7 +838,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
             }
         }
     } else if (warp < 4) {
-        const float alpha = g.tensorP ? g.tensorP[0] * g.tensorQ[0] : 1.f;
+        const Factors f = factorsOf(g);
         const unsigned int accFree0 = addrIn(accFree, 0);
         const unsigned int staging = stage0 + S::stages * S::stageBytes + warp * S::stagingBytes;
         int done = 0;
@@ -808,11 +851,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
             const unsigned int acc = tmem + buf * S::accStep + (static_cast<unsigned int>(warp * 32) << 16);
             const long long row0 = static_cast<long long>(tp) * 256 + rank * 128 + warp * 32, q0 = static_cast<long long>(tq) * 256;
             if (g.outTag == T_F16) {
-                pairEpilogue<__half>(g, &mapOut, staging, acc, buf, row0, q0, alpha, accFree0, lane);
+                pairEpilogue<__half>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
             } else if (g.outTag == T_BF16) {
-                pairEpilogue<__nv_bfloat16>(g, &mapOut, staging, acc, buf, row0, q0, alpha, accFree0, lane);
+                pairEpilogue<__nv_bfloat16>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
             } else {
-                pairEpilogue<float>(g, &mapOut, staging, acc, buf, row0, q0, alpha, accFree0, lane);
+                pairEpilogue<float>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
             }
         }
     }

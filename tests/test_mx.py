@@ -428,6 +428,31 @@ def test_matmul_is_exact_where_sums_are(dev, fmt, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(5, 40, 64), (5, 300, 2048), (129, 200, 512), (1600, 1800, 128), (1537, 1701, 300)])
+@pytest.mark.parametrize("ta,tb", [(2.0 ** -75, 2.0 ** -75), (2.0 ** -75 * 1.37, 2.0 ** -80 * 1.91), (2.0 ** 65, 2.0 ** 65), (2.0 ** 70 * 1.7, 2.0 ** 59),
+                                   (2.0 ** -100, 2.0 ** 100), (3e38, 2e-38), (2.0 ** -149, 2.0 ** 20), (2.0 ** -140 * 3, 2.0 ** 10 * 1.3),
+                                   (2.0 ** -126, 2.0 ** -126), (3e38, 3e38), (2.0 ** -149, 2.0 ** -149)])
+def test_matmul_over_the_range_of_the_tensor_scales(dev, m, n, k, ta, tb):
+    """Their product may leave 32 bits where the results do not; rows of zeros stay zeros."""
+    (a, va), (b, vb) = random_held(A.NVFP4, m, k, m + 5, spread=6), random_held(A.NVFP4, n, k, n + 6, spread=6)
+    for h, v, t in ((a, va, ta), (b, vb, tb)):
+        v *= float(np.float32(t)) / float(h.tensor[0])
+        h.tensor[0] = float(np.float32(t))
+        v[1] = 0
+        h.codes[:h.rows * h.ld].view(h.rows, h.ld)[1] = 0
+    # what is above the largest number by more than half a step, and by what a sum may be off (see check_product)
+    above = np.abs(va @ vb.T) - (-(-k // 64) + 2) * 2.0 ** -23 * (np.abs(va) @ np.abs(vb).T)
+    for dtype, pad in ((A.F32, 0), (A.BF16, 8), (A.F16, 3)):
+        out = torch.full((m, n + pad), 7.0, dtype=TYPES[dtype], device="cuda")
+        dev.mx_matmul(a.m, b.m, out.data_ptr(), dtype, out.stride(0))
+        got = out[:, :n].double().cpu().numpy()
+        check_product(got, va, vb, dtype)
+        assert (got[1] == 0).all() and (got[:, 1] == 0).all()
+        info = torch.finfo(TYPES[dtype])
+        assert np.isinf(got[above > info.max * (1 + info.eps)]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(20, 150, 200), (1700, 1601, 200)])
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_matmul_keeps_nan_to_its_rows(dev, fmt, m, n, k):
