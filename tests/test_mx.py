@@ -279,6 +279,74 @@ def test_quantize_with_a_given_tensor_scale(dev, dtype, t):
     assert h.tensor.tolist() == [float(np.float32(t)), -1.0]  # read, not written
 
 
+def steps_from(x, steps):
+    """32-bit numbers so many units in the last place from x."""
+    return (np.asarray(x, np.float32)[..., None].view(np.int32) + np.asarray(steps, np.int32)).view(np.float32)
+
+
+def next_to_borders(t, scales):
+    """Rows of blocks for the tensor scale t: each block's largest element gives it one of `scales`, its others lie next
+    to the borders between the codes of 4 bits."""
+    e4m3 = O.e4m3_values()[scales].astype(np.float32)
+    d = e4m3 * np.float32(t)  # rounded to 32 bits, as the definition says
+    v = steps_from(d[:, None] * np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float32), range(-3, 4)).reshape(len(d), 49)
+    x = np.zeros((len(d), 64), np.float32)
+    x[:, ::16] = (6 * d)[:, None]
+    x[:, [i for i in range(64) if i % 16][:49]] = v * np.where(np.arange(49) % 3 == 1, -1, 1).astype(np.float32)
+    return x
+
+
+def next_to_scales(t):
+    """One block a row, whose largest element lies next to a border between two of e4m3's numbers."""
+    values = O.e4m3_values()[:127]
+    top = steps_from((np.float32(6) * np.float32(t)) * ((values[1:] + values[:-1]) / 2).astype(np.float32), range(-3, 4)).reshape(-1)
+    x = np.zeros((len(top), 16), np.float32)
+    x[:, 5] = top
+    return x
+
+
+def check_quotients(dev, x, t):
+    h = Held(A.NVFP4, x.shape[0], x.shape[1], A.MX_SCALES_ROWS, t=t)
+    src = torch.from_numpy(x).cuda()
+    dev.mx_quantize(src.data_ptr(), A.F32, x.shape[1], h.m, tensor_scale_given=True)
+    h.check(O.quantize(x, A.NVFP4, t=np.float32(t)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("exponent", [0, -30, 21, -100, 90])
+@pytest.mark.parametrize("eighths", range(8, 17))
+def test_quotients_of_the_divisors_that_could_be_misrounded(dev, eighths, exponent):
+    """Full-width divisors for which a rounded quotient may fall on a border although the quotient does not: those within
+    some units in the last place of a multiple of 1/8.  Every one of them, against correctly rounded quotients."""
+    near = steps_from(np.float32(eighths / 8), range(-64, 65))
+    for d in near:
+        t = float(d) * 2.0 ** exponent
+        check_quotients(dev, next_to_borders(t, np.array([56, 48, 64])), t)  # scales of 1, 0.5 and 2: d is t
+    for six in near:
+        for t in steps_from(six / np.float32(6) * np.float32(2.0 ** exponent), (-1, 0, 1)):
+            if np.float32(6) * t == np.float32(float(six) * 2.0 ** exponent):
+                check_quotients(dev, next_to_scales(t), float(t))
+                break
+
+
+@pytest.mark.gpu
+def test_quotients_of_random_divisors(dev):
+    rng = np.random.default_rng(21)
+    for _ in range(150):
+        t = float(np.float32(rng.uniform(1, 2) * 2.0 ** rng.integers(-30, 20)))
+        check_quotients(dev, next_to_borders(t, np.arange(1, 127)), t)
+        check_quotients(dev, next_to_scales(t), t)
+
+
+def test_borders_of_the_codes_and_their_neighbours():
+    """The inputs of the tests above reach both sides of every border, and the border itself."""
+    t = np.float32(1.5)
+    q = O.quantize(next_to_borders(t, np.array([56])), A.NVFP4, t=t)["codes"][0] & 7
+    assert set(q) == set(range(8))
+    s = O.quantize(next_to_scales(t), A.NVFP4, t=t)["scales"]
+    assert set(s.reshape(-1)) == set(range(127))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_quantize_extreme_magnitudes(dev, fmt):
