@@ -154,10 +154,24 @@ __device__ __forceinline__ unsigned int addrIn(unsigned int addr, unsigned int r
 __device__ __forceinline__ void expectBytes(unsigned int bar, unsigned int bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void drain(unsigned int bar, unsigned int parity) {
+// After a wait that gave up: what was issued goes on all the same -- loads write shared memory, products read it and write
+// tensor memory, commits arrive at barriers -- so a CTA frees and leaves nothing before all of it is done.  The barriers
+// say when: use number n of a barrier completes its phase n.  These waits have the same limit.
+__device__ __forceinline__ void drain(unsigned int bar, int use) {
     const long long start = clock64();
-    while (!barTry(bar, parity) && clock64() - start < 4000000000ll) {
+    while (!barTry(bar, use & 1) && clock64() - start < 4000000000ll) {
     }
+}
+// the last use of each of a ring of barriers, `uses` in all
+__device__ __forceinline__ void drainRing(unsigned int bars, int stages, int uses) {
+    for (int i = max(0, uses - stages); i < uses; ++i) drain(bars + 8 * (i % stages), i / stages);
+}
+__device__ __forceinline__ void storeIn(unsigned int addr, unsigned int rank, int v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addrIn(addr, rank)), "r"(v) : "memory");
+}
+// `bytes` that will not come are counted as if they had
+__device__ __forceinline__ void forgoBytes(unsigned int bar, unsigned int bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void loadTile(unsigned int dst, const CUtensorMap* map, int x, int y, unsigned int bar) {
@@ -506,10 +520,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     allowNext();
     const unsigned int acc = tmemBase, scaleCol = tmemBase + BN;
+    int issued = 0;  // stages whose loads (warp 4) or products (warp 5) have been issued
 
     if (warp == 4) {
         const long long scaleTileP = p0 / 128, scaleTileQ = q0 / 128;
-        int s = 0, phase = 1, issued = 0;
+        int s = 0, phase = 1;
         for (; issued < n; ++issued) {
             if (!__all_sync(0xFFFFFFFFu, issued < stages || barWait(empty + 8 * s, phase, stalled))) break;
             if (electOne()) {
@@ -527,15 +542,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
             __syncwarp();
             if (++s == stages) s = 0, phase ^= 1;
         }
-        // a wait that gave up leaves copies in flight: they write this CTA's memory, so it stays until they have
-        if (*stalled) {
-            for (int i = max(0, issued - stages); i < issued; ++i) drain(full + 8 * (i % stages), (i / stages) & 1);
-        }
     } else if (warp == 5) {
         const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesP);
         const unsigned long long ds0 = scaleDesc(stage0 + S::bytesP + S::bytesQ);
         int s = 0, phase = 0, before = 0, beforePhase = 0;  // before: the stage scaleBufs ago
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < n; ++i, ++issued) {
             if (!__all_sync(0xFFFFFFFFu, barWait(full + 8 * s, phase, stalled))) break;
             // the scales' columns are free once the products that read them are done: nothing else orders a copy behind them
             if (i >= S::scaleBufs) {
@@ -622,6 +633,14 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (*stalled) {  // all warps see the same: none sets it behind the barrier
+        if (warp == 4) drainRing(full, stages, issued);
+        if (warp == 5) {
+            drainRing(empty, stages, issued);
+            if (issued == n) drain(done, 0);
+        }
+        __syncthreads();
+    }
     if (warp == 5) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmemBase), "r"(S::cols) : "memory");
@@ -734,7 +753,8 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
     extern __shared__ unsigned char raw[];
     __shared__ unsigned long long bars[2 * S::stages + 2];
     __shared__ unsigned int tmemBase;
-    __shared__ int stalledWord;
+    __shared__ int stalledWord, peerStalled;
+    __shared__ int loadsOf[2], productsDone, tilesDone;  // of each CTA's loads, and of the first CTA's products: stages issued
     volatile int* stalled = &stalledWord;
     const unsigned int stage0 = (smemAddr(raw) + 1023u) & ~1023u;
     const unsigned int full = smemAddr(bars), empty = full + 8 * S::stages, accFull = empty + 8 * S::stages, accFree = accFull + 8;
@@ -755,7 +775,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
         barInit(accFull, 1);
         barInit(accFree, 8);  // four epilogue warps of both CTAs
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        stalledWord = 0;
+        stalledWord = peerStalled = 0;
     }
     afterLast();
     if (warp == 5) {
@@ -793,14 +813,13 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
                 if (++s == S::stages) s = 0, phase ^= 1;
             }
         }
-        if (*stalled && rank == 0) {  // copies in flight write both CTAs' memory, which stays until they have
-            for (int i = max(0, issued - S::stages); i < issued; ++i) drain(full + 8 * (i % S::stages), (i / S::stages) & 1);
-        }
+        if (lane < 2) storeIn(smemAddr(&loadsOf[rank]), lane, issued);
     } else if (warp == 5 && rank == 0) {
         const unsigned long long dp0 = operandDesc(stage0), dq0 = operandDesc(stage0 + S::bytesSide);
         const unsigned long long ds0 = scaleDesc(stage0 + 2 * S::bytesSide);
         int s = 0, phase = 0, it = 0, done = 0;
         int before = 0, beforePhase = 0;  // the stage, scaleBufs ago, whose products must be done with their scales
+        int whole = 0;  // tiles whose products have all been issued
         bool ok = true;
         for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs, ++done) {
             const unsigned int acc = tmem + (done & 1) * S::accStep;
@@ -835,7 +854,12 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
                 }
                 __syncwarp();
                 if (++s == S::stages) s = 0, phase ^= 1;
+                if (kt + 1 == g.ktiles) ++whole;
             }
+        }
+        if (lane < 2) {
+            storeIn(smemAddr(&productsDone), lane, it);
+            storeIn(smemAddr(&tilesDone), lane, whole);
         }
     } else if (warp < 4) {
         const Factors f = factorsOf(g);
@@ -861,8 +885,36 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
     }
     if (warp < 4 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the last stores are through
     __syncwarp();
+    if (*stalled && lane == 0) storeIn(smemAddr(&peerStalled), rank ^ 1, 1);
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     clusterSync();  // neither CTA leaves while the other's products, copies or arrivals reach into it
+    if (*stalled || *const_cast<volatile int*>(&peerStalled)) {  // both CTAs see the same
+        if (warp == 4 && rank == 0) {
+            // the loads of both CTAs are counted here; one of them may have gone on for some stages
+            constexpr unsigned int half = 2 * S::bytesSide + 3 * S::scaleBytes;
+            const int n0 = loadsOf[0], n1 = loadsOf[1];
+            drainRing(full, S::stages, min(n0, n1));
+            for (int i = min(n0, n1); i < max(n0, n1); ++i) {
+                const unsigned int bar = full + 8 * (i % S::stages);
+                if (lane == 0) {
+                    if (n1 > n0) {
+                        expectBytes(bar, half);
+                    } else {
+                        forgoBytes(bar, half);
+                    }
+                }
+                __syncwarp();
+                drain(bar, i / S::stages);
+            }
+        }
+        if (warp == 5) {
+            drainRing(empty, S::stages, productsDone);
+            if (tilesDone > 0) drain(accFull, tilesDone - 1);
+        }
+        __syncwarp();
+        clusterSync();
+    }
     if (warp == 5) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmemBase), "r"(S::cols) : "memory");
