@@ -1043,9 +1043,6 @@ void launchTileOf(Context* ctx, const b200c_mx_matrix& p, const b200c_mx_matrix&
     g.tilesQ = static_cast<int>((q.rows + BN - 1) / BN);
     const long long tiles = static_cast<long long>(g.tilesP) * g.tilesQ;
     g.split = splitOf(ctx, tiles, g.ktiles, BN);
-#ifdef FORCE_SPLIT
-    if (const char* e = std::getenv("MXSPLIT")) if (std::atoi(e)) g.split = std::min(g.ktiles, std::atoi(e));
-#endif
     if (tiles * g.split > 0x7FFFFFFFll) throw BadArg("the product has too many tiles");
     launchClusters(ctx, mxMatmulKernel<BN, NV>, static_cast<unsigned int>(tiles * g.split), static_cast<unsigned int>(g.split),
                    S::smemBytes, mapOf(p, 128), mapOf(q, BN), g);
