@@ -204,7 +204,9 @@ typedef void* (*b200c_alloc_fn)(void* user, size_t bytes);
 typedef void (*b200c_free_fn)(void* user, void* ptr);
 B200C_API int b200c_set_allocator(b200c_ctx* ctx, b200c_alloc_fn alloc_fn, b200c_free_fn free_fn, void* user);
 /* Use `stream` (a cudaStream_t) for all later work of this context; NULL
- * restores the context's own stream.                                          */
+ * restores the context's own stream.  Nothing orders the work queued before with that on the
+ * new stream: the caller synchronises, or orders the two by an event -- above all after calls with
+ * B200C_FOLD_ASYNC, whose workspace the next fold uses again.                  */
 B200C_API int b200c_set_stream(b200c_ctx* ctx, void* stream);
 B200C_API void* b200c_get_stream(b200c_ctx* ctx);
 /* Waits for the context's stream (and its transfer stream, if used) and reports device-side errors. */

@@ -620,7 +620,9 @@ class CudaBackend:
 
     def set_stream(self, stream):
         """All later work of this backend goes to `stream` (a cudaStream_t as an integer, e.g. a torch stream's
-        cuda_stream; 0 is CUDA's default stream).  None: back to the backend's own stream."""
+        cuda_stream; 0 is CUDA's default stream).  None: back to the backend's own stream.  Work queued before is not waited
+        for, and nothing orders it before the work on the new stream: whoever changes the stream synchronises or orders the
+        two by an event, above all after folds that return before they are done, whose workspace the next fold uses again."""
         handle = None if stream is None else int(stream) or 1  # cudaStreamLegacy: a null handle means the own stream
         raise_for(self.lib.b200c_set_stream(self.ctx, handle), self._err())
 
