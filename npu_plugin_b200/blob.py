@@ -72,8 +72,7 @@ class ShardFolder:
         self.folded_offsets, self.folded_sizes = [], []
         at = 0
         for d in decls:
-            if any(t.kind in (A.X_QUANTIZE_MX, A.X_DEQUANTIZE_MX) and isinstance(s, np.ndarray) for t in d.transforms
-                   for s in (t.side0, t.side1)):
+            if any(isinstance(s, np.ndarray) for t in d.transforms for s in (t.side0, t.side1)):
                 raise ValueError(f"{d.name}: scales of a constant that is folded on the device have to lie there")
             final = backend.infer_type(d.base_type, d.transforms)
             size = final.getTotalAllocSize()

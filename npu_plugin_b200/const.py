@@ -431,6 +431,34 @@ class ResidentContent:
             self.done()
 
 
+class DeviceSides:
+    """The side arrays of lists whose result stays on the device: they have to lie there too while the fold runs."""
+
+    def __init__(self, backend):
+        self._backend, self._held = backend, []  # (device buffer, host array, written by the fold)
+
+    def move(self, chain, transforms):
+        """Device buffers in the place of the host arrays of `chain`, which chain_to_c made of `transforms`."""
+        for x, t in zip(chain, transforms):
+            for name in ("side0", "side1"):
+                host = getattr(t, name)
+                if isinstance(host, np.ndarray):
+                    self._held.append((self._backend.dev_alloc(host.nbytes), host, t.kind in t.WRITES_SIDES))
+                    self._backend.upload(self._held[-1][0], host)
+                    setattr(x, name, self._held[-1][0])
+
+    def fetch(self):
+        """What the fold wrote, into the host arrays."""
+        for dev, host, written in self._held:
+            if written:
+                host.view(np.uint8).reshape(-1)[:] = self._backend.download(dev, host.nbytes)
+
+    def release(self):
+        for dev, _, _ in self._held:
+            self._backend.dev_free(dev)
+        self._held = []
+
+
 # --------------------------------------------------------------------------- backend (CUDA library)
 class CudaBackend:
     """Calls libb200const.so; one b200c_ctx per backend object."""
@@ -498,16 +526,9 @@ class CudaBackend:
         out = self.dev_alloc(cap)
         ot = out_type_slot(max(q_slots_of(final), quick_q_of(base_type, transforms)), keep)
         nb = C.c_size_t()
-        sides = []  # (device buffer, host array, written by the fold)
+        sides = DeviceSides(self)
         try:
-            # the result stays on the device, and so do the side arrays while the fold runs
-            for x, t in zip(ch, transforms):
-                for name in ("side0", "side1"):
-                    host = getattr(t, name)
-                    if isinstance(host, np.ndarray):
-                        sides.append((self.dev_alloc(host.nbytes), host, t.kind in t.WRITES_SIDES))
-                        self.upload(sides[-1][0], host)
-                        setattr(x, name, sides[-1][0])
+            sides.move(ch, transforms)
             self.fill_zero(out, cap)
             if isinstance(data, ResidentContent):
                 src, n, on_dev = data.buf, data.nbytes, 1
@@ -517,15 +538,12 @@ class CudaBackend:
             rc = self.lib.b200c_fold(self.ctx, C.byref(bt), src, n, int(is_splat), on_dev, ch, len(transforms), out, cap, 1,
                                      C.byref(nb), C.byref(ot), 0)
             raise_for(rc, self._err())
-            for dev, host, written in sides:
-                if written:
-                    host.view(np.uint8).reshape(-1)[:] = self.download(dev, host.nbytes)
+            sides.fetch()
         except Exception:
             self.dev_free(out)
             raise
         finally:
-            for dev, _, _ in sides:
-                self.dev_free(dev)
+            sides.release()
         t = NDType.from_c(ot)
         return ResidentContent(self, t, out, max(t.getTotalAllocSize(), nb.value), nb.value)
 

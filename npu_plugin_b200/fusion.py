@@ -18,7 +18,7 @@ import ctypes as C
 import numpy as np
 
 from . import _cabi as A
-from .const import NDType, chain_to_c, raise_for
+from .const import DeviceSides, NDType, chain_to_c, raise_for
 
 
 class FusedConstant:
@@ -55,6 +55,7 @@ def fuse_constants(backend, weight_table=None, weights=None, weights_sm=None, ac
     lib, ctx = backend.lib, backend.ctx
     fused_dev = backend.dev_alloc(max(1, total))
     staged, keep = [], []
+    sides = DeviceSides(backend)
     try:
         backend.fill_zero(fused_dev, max(1, total))
         n = len(present)
@@ -67,6 +68,7 @@ def fuse_constants(backend, weight_table=None, weights=None, weights_sm=None, ac
             backend.upload(d, raw)
             bt = p._baseType.to_c(keep)
             ch = chain_to_c(p.getTransformations(), keep)
+            sides.move(ch, p.getTransformations())
             keep += [bt, ch]
             it = items[k]
             it.base = C.pointer(bt)
@@ -81,7 +83,9 @@ def fuse_constants(backend, weight_table=None, weights=None, weights_sm=None, ac
         if n:
             raise_for(lib.b200c_fold_batch(ctx, items, n, 1, 1, 0), lib.b200c_last_error())
         data = backend.download(fused_dev, total)
+        sides.fetch()
     finally:
+        sides.release()
         backend.dev_free(fused_dev)
         for d in staged:
             backend.dev_free(d)

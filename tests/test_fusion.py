@@ -132,3 +132,82 @@ def test_gpu_section_writer(gpu, align):
     consts = [blob_host[o:o + s] for _, o, s, _ in table]
     want, offs = (fusion_oracle.graph_schema_section if align == 8 else fusion_oracle.elf_section)(consts)
     assert sec.offsets == offs and np.array_equal(sec.data, want)
+
+
+# --------------------------------------------------------------------------- parts that write side arrays
+def quantised_parts(backend):
+    rng = np.random.default_rng(31)
+    h = rng.normal(0, 1, (16, 64)).astype(np.float16)
+    w = rng.normal(0, 1, (8, 16, 3, 3)).astype(np.float32)
+    mx = ContentAttr.get(h, backend=backend).quantizeMx(A.NVFP4).swizzleConstant(5, 3)
+    synth = ContentAttr.get(w, backend=backend).quantizeSynth(A.QSYNTH_ASYM_U4).convertElemType(A.UI8)
+    return synth, mx
+
+
+def test_fusion_gives_the_device_no_host_address():
+    from npu_plugin_b200.fusion import fuse_constants
+    from test_abi_and_host import HostOnly
+
+    class Recorder(HostOnly):
+        """Device memory that is only counted; a batched fold that looks at its side arrays."""
+        ctx = None
+
+        def __init__(self):
+            super().__init__()
+            self.real, self.lib, self.at, self.blocks = self.lib, self, 1 << 40, {}
+            self.b200c_infer_type, self.b200c_last_error = self.real.b200c_infer_type, self.real.b200c_last_error
+            self.b200c_insert_position = self.real.b200c_insert_position
+
+        def dev_alloc(self, nbytes):
+            self.at += 1 << 20
+            self.blocks[self.at] = nbytes
+            return self.at
+
+        def dev_free(self, ptr):
+            del self.blocks[ptr]
+
+        def fill_zero(self, ptr, nbytes):
+            pass
+
+        def upload(self, ptr, array):
+            assert array.nbytes <= self.blocks[ptr]
+
+        def download(self, ptr, nbytes):
+            return np.full(nbytes, 3, np.uint8)
+
+        def b200c_fold_batch(self, ctx, items, n, data_on_device, out_on_device, flags):
+            assert out_on_device
+            given = [p for i in range(n) for k in range(items[i].n) for p in (items[i].chain[k].side0, items[i].chain[k].side1) if p]
+            assert len(given) == 4 and all(p in self.blocks for p in given)
+            return A.OK
+
+    r = Recorder()
+    synth, mx = quantised_parts(r)
+    fuse_constants(r, weights=mx, weights_sm=synth)
+    assert not r.blocks
+    for side in (synth.sideScales, synth.sideZeroPoints, mx.mxScales, mx.mxTensorScale):
+        assert (side.view(np.uint8) == 3).all()
+
+
+@pytest.mark.gpu
+def test_fused_parts_write_their_side_arrays(gpu):
+    from npu_plugin_b200.fusion import fuse_constants
+    synth, mx = quantised_parts(gpu)
+    fused = fuse_constants(gpu, weights=mx, weights_sm=synth)
+    got = [x.copy() for x in (synth.sideScales, synth.sideZeroPoints, mx.mxScales, mx.mxTensorScale)]
+    want = [np.array(a.fold().copyTo()) for a in (mx, synth)]
+    assert np.array_equal(fused.data, np.concatenate(want))
+    for g, x in zip(got, (synth.sideScales, synth.sideZeroPoints, mx.mxScales, mx.mxTensorScale)):
+        assert np.array_equal(g, x) and (g != 0).any()
+
+
+def test_host_arrays_are_refused_where_the_fold_runs_on_the_device():
+    from npu_plugin_b200.blob import ConstantDecl, ShardFolder
+    from npu_plugin_b200.const import Transform
+    from test_abi_and_host import HostOnly
+
+    class Backend(HostOnly):
+        ctx = None
+    d = ConstantDecl("w", NDType((8, 64), A.F16), [Transform(A.X_QUANTIZE_SYNTH, i0=A.QSYNTH_SYM_I8, side0=np.zeros(8, np.float32))], 1024)
+    with pytest.raises(ValueError, match="have to lie there"):
+        ShardFolder(Backend(), [d])
