@@ -821,6 +821,11 @@ class ContentAttr:
     def withBackend(self, backend):
         return ContentAttr(self._base, self._baseType, self._isSplat, self._transforms, backend)
 
+    def _typeAt(self, kind):
+        """The type that a new transformation of `kind` will see: some stay behind it (swizzling, sparsification)."""
+        pos = self._backend.insert_position([t.kind for t in self._transforms], kind)
+        return self._backend.infer_type(self._baseType, self._transforms[:pos])
+
     # -- ContentAttr::addTransformation (content.cpp:305-331)
     def addTransformation(self, t):
         kinds = [x.kind for x in self._transforms]
@@ -927,7 +932,7 @@ class ContentAttr:
     def quantizeSynth(self, scheme):
         """Synthetic per-output-channel quantiser (no reference counterpart); the per-channel
         scales / zero points land in the returned attribute's `.sideScales` / `.sideZeroPoints`."""
-        oc = self.getType().shape[0]
+        oc = self._typeAt(A.X_QUANTIZE_SYNTH).shape[0]
         s0 = np.zeros(oc, dtype=np.float32)
         s1 = np.zeros(oc, dtype=np.int32)
         out = self.addTransformation(Transform(A.X_QUANTIZE_SYNTH, i0=scheme, side0=s0, side1=s1))
@@ -938,7 +943,7 @@ class ContentAttr:
         blocks run along the innermost memory dimension, a multiple of 32.  The scales [rows, blocks] land in the
         returned attribute's `.mxScales`, for nvfp4 the tensor scale (found from the data when 0) and the largest
         magnitude in `.mxTensorScale`."""
-        mem = self.getType().getMemShape()
+        mem = self._typeAt(A.X_QUANTIZE_MX).getMemShape()
         cols = mem[-1] if mem else 0
         rows = int(np.prod(mem[:-1], dtype=np.int64))
         s0 = np.zeros((rows, -(-cols // (32 if fmt == A.MXFP4 else 16))), np.uint8)
@@ -951,7 +956,7 @@ class ContentAttr:
         s0 = None if scales is None else np.ascontiguousarray(scales, np.uint8)
         s1 = None if tensorScale is None else np.ascontiguousarray(tensorScale, np.float32).reshape(-1)
         if s0 is not None:
-            mem = self.getType().getMemShape()
+            mem = self._typeAt(A.X_DEQUANTIZE_MX).getMemShape()
             want = int(np.prod(mem[:-1], dtype=np.int64)) * -(-(mem[-1] if mem else 0) // (32 if fmt == A.MXFP4 else 16))
             if s0.size != want:
                 raise ConstError(f"DequantizeMx: {s0.size} scales for {want} blocks")

@@ -69,6 +69,21 @@ def test_wrong_numbers_of_scales_are_refused():
         attr.dequantizeMx(A.NVFP4, A.F16, scales=np.zeros(31, np.uint8), tensorScale=[1.0])
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_scales_have_the_shape_of_what_is_quantised(fmt):
+    """Swizzling stays behind, whichever was asked for first."""
+    host = HostOnly()
+    w = ContentAttr.get(np.zeros((8, 256), np.float16), is_splat=False, backend=host)
+    for q in (w.quantizeMx(fmt), w.quantizeMx(fmt).swizzleConstant(5, 3), w.swizzleConstant(5, 3).quantizeMx(fmt)):
+        assert q.mxScales.shape == (8, 256 // O.BLOCK[fmt])
+    stored = ContentAttr.get(np.zeros(1024, np.uint8), NDType((8, 256), A.F4E2M1), False, host)
+    scales = np.zeros((8, 256 // O.BLOCK[fmt]), np.uint8)
+    back = stored.swizzleConstant(5, 3).dequantizeMx(fmt, A.F16, scales, [1.0] if fmt == A.NVFP4 else None)
+    assert [t.kind for t in back.getTransformations()] == [A.X_DEQUANTIZE_MX, A.X_SWIZZLE_CONSTANT]
+    s = w.swizzleConstant(5, 3).quantizeSynth(A.QSYNTH_SYM_I8)
+    assert s.sideScales.shape == s.sideZeroPoints.shape == (8,)
+
+
 def test_two_transformations_with_their_own_scales_are_not_one():
     s = np.zeros((8, 2), np.uint8)
     assert Q(A.MXFP4, side0=s) == Q(A.MXFP4, side0=s)
@@ -233,6 +248,16 @@ def test_conv_weight_chain(gpu, oracle, fmt):
         back = q.dequantizeMx(fmt, elem).fold()
         assert back.getType().dtype == elem and tuple(back.getType().order) == tuple(DimsOrder.OYXI)
         np.testing.assert_array_equal(back.getValues(), want["values"].astype(np.float32).astype(dt).reshape(-1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_swizzled_first_and_quantised_then(gpu, fmt):
+    a = ContentAttr.get(np.random.default_rng(8).normal(0, 1, (24, 96)).astype(np.float16), backend=gpu)
+    one, other = a.quantizeMx(fmt).swizzleConstant(5, 3), a.swizzleConstant(5, 3).quantizeMx(fmt)
+    np.testing.assert_array_equal(one.fold().copyTo(), other.fold().copyTo())
+    np.testing.assert_array_equal(one.mxScales, other.mxScales)
+    assert (one.mxScales != 0).all()
 
 
 @pytest.mark.gpu
