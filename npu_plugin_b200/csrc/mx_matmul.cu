@@ -30,7 +30,7 @@ namespace {
 struct MxMatmulParams {
     const unsigned char* scalesP;
     const unsigned char* scalesQ;
-    const float* tensorP;  // nullptr: 1
+    const float* tensorP;  // nvfp4
     const float* tensorQ;
     long long rowsP, rowsQ, k;
     long long chunks;      // tiles of 4 blocks along k: 512 bytes of scales each, per 128 rows
@@ -157,13 +157,13 @@ __device__ __forceinline__ void expectBytes(unsigned int bar, unsigned int bytes
 // After a wait that gave up: what was issued goes on all the same -- loads write shared memory, products read it and write
 // tensor memory, commits arrive at barriers -- so a CTA frees and leaves nothing before all of it is done.  The barriers
 // say when: use number n of a barrier completes its phase n.  These waits have the same limit.
-__device__ __forceinline__ void drain(unsigned int bar, int use) {
+__device__ __noinline__ void drain(unsigned int bar, int use) {
     const long long start = clock64();
     while (!barTry(bar, use & 1) && clock64() - start < 4000000000ll) {
     }
 }
 // the last use of each of a ring of barriers, `uses` in all
-__device__ __forceinline__ void drainRing(unsigned int bars, int stages, int uses) {
+__device__ __noinline__ void drainRing(unsigned int bars, int stages, int uses) {
     for (int i = max(0, uses - stages); i < uses; ++i) drain(bars + 8 * (i % stages), i / stages);
 }
 __device__ __forceinline__ void storeIn(unsigned int addr, unsigned int rank, int v) {
@@ -338,28 +338,38 @@ __device__ __forceinline__ float toOut<float>(float v) {
 // zeros.  Sums are 0 or lie within 2^-20 .. 2^54 (codes of 0.5 with scales of 2^-9 on both sides; 36 * 448^2 for each
 // of 2^31 elements), so the exponent is shared out evenly: a product with the first factor is below the normal numbers
 // only where the result is 0 anyway, and above the largest only where the result is, too.
-struct Factors {
+template <bool NV>
+struct Factors {};  // mxfp4 has none
+template <>
+struct Factors<true> {
     float first, second;
 };
-__device__ __noinline__ Factors farFactors(float tp, float tq) {
+__device__ __noinline__ Factors<true> farFactors(float tp, float tq) {
     int ep, eq;
     const float m = frexpf(tp, &ep) * frexpf(tq, &eq);
     // beyond these the result is 0 or infinity whatever the sum
     const int e = min(max(ep + eq, -212), 200);
-    return Factors{ldexpf(m, e / 2), ldexpf(1.f, e - e / 2)};
+    return Factors<true>{ldexpf(m, e / 2), ldexpf(1.f, e - e / 2)};
 }
-__device__ __forceinline__ Factors factorsOf(const MxMatmulParams& g) {
-    if (!g.tensorP) return Factors{1.f, 1.f};
+template <bool NV>
+__device__ __forceinline__ Factors<NV> factorsOf(const MxMatmulParams&) {
+    return {};
+}
+template <>
+__device__ __forceinline__ Factors<true> factorsOf<true>(const MxMatmulParams& g) {
     const float tp = g.tensorP[0], tq = g.tensorQ[0], product = tp * tq;
     const bool normal = fabsf(product) >= 1.17549435e-38f && fabsf(product) <= 3.402823466e38f;
     // a scale that is 0, infinite or NaN has only the product that it has
-    if (normal || tp == 0.f || tq == 0.f || !(fabsf(tp) <= 3.402823466e38f && fabsf(tq) <= 3.402823466e38f)) return Factors{product, 1.f};
+    if (normal || tp == 0.f || tq == 0.f || !(fabsf(tp) <= 3.402823466e38f && fabsf(tq) <= 3.402823466e38f)) return {product, 1.f};
     return farFactors(tp, tq);
 }
 
 // N sums times both factors, two at a time
 template <int N>
-__device__ __forceinline__ void scaled(const Factors& f, float* v) {
+__device__ __forceinline__ void scaled(const Factors<false>&, float*) {
+}
+template <int N>
+__device__ __forceinline__ void scaled(const Factors<true>& f, float* v) {
     static_assert(N % 2 == 0, "pairs");
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
@@ -388,8 +398,8 @@ __device__ __forceinline__ void storeAcross(const MxMatmulParams& g, long long p
             if (i < left) *at = toOut<T>(v[i]);
     }
 }
-template <class T, int BN>
-__device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int acc, long long p, long long q0, const Factors& f) {
+template <class T, int BN, bool NV>
+__device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int acc, long long p, long long q0, const Factors<NV>& f) {
     constexpr int n = BN < 32 ? BN : 32;
 #pragma unroll 1
     for (int c = 0; c < BN && q0 + c < g.rowsQ; c += n) {
@@ -408,9 +418,9 @@ __device__ __forceinline__ void epilogue(const MxMatmulParams& g, unsigned int a
 // up its share of the columns, in the order of the ranks, so that the result is the same on every run.  A thread takes
 // four rows at a time, and 16 loads from the cluster's memory are under way at once: with one column at a time the
 // waiting for them took longer than the product itself.
-template <class T, int BN, int MOST>
+template <class T, int BN, int MOST, bool NV>
 __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0,
-                                            long long q0, const Factors& f) {
+                                            long long q0, const Factors<NV>& f) {
     constexpr int most = 16 / MOST;
     const int c0 = static_cast<int>(rank) * BN / g.split, c1 = (static_cast<int>(rank) + 1) * BN / g.split;
     const int row = thread % 32 * 4;
@@ -467,15 +477,15 @@ __device__ __forceinline__ void joinColumns(const MxMatmulParams& g, unsigned in
     }
 }
 
-template <class T, int BN>
+template <class T, int BN, bool NV>
 __device__ __forceinline__ void join(const MxMatmulParams& g, unsigned int sums, unsigned int rank, int thread, long long p0, long long q0,
-                                     const Factors& f) {
+                                     const Factors<NV>& f) {
     if (g.split <= 2) {
-        joinColumns<T, BN, 2>(g, sums, rank, thread, p0, q0, f);
+        joinColumns<T, BN, 2, NV>(g, sums, rank, thread, p0, q0, f);
     } else if (g.split <= 4) {
-        joinColumns<T, BN, 4>(g, sums, rank, thread, p0, q0, f);
+        joinColumns<T, BN, 4, NV>(g, sums, rank, thread, p0, q0, f);
     } else {
-        joinColumns<T, BN, 8>(g, sums, rank, thread, p0, q0, f);
+        joinColumns<T, BN, 8, NV>(g, sums, rank, thread, p0, q0, f);
     }
 }
 
@@ -585,7 +595,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         }
     }
     __syncwarp();
-    const Factors f = factorsOf(g);  // before the wait, which hides its loads
+    const Factors<NV> f = factorsOf<NV>(g);  // before the wait, which hides its loads
     const bool finished = warp < 4 && __all_sync(0xFFFFFFFFu, barWait(done, 0, stalled) && !*stalled);  // the reads are the whole warp's
     const unsigned int mine = acc + (static_cast<unsigned int>(warp * 32) << 16);
     const int row = warp * 32 + lane;
@@ -593,11 +603,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
     if (g.split == 1) {
         if (finished) {
             if (g.outTag == T_F16) {
-                epilogue<__half, BN>(g, mine, p0 + row, q0, f);
+                epilogue<__half, BN, NV>(g, mine, p0 + row, q0, f);
             } else if (g.outTag == T_BF16) {
-                epilogue<__nv_bfloat16, BN>(g, mine, p0 + row, q0, f);
+                epilogue<__nv_bfloat16, BN, NV>(g, mine, p0 + row, q0, f);
             } else {
-                epilogue<float, BN>(g, mine, p0 + row, q0, f);
+                epilogue<float, BN, NV>(g, mine, p0 + row, q0, f);
             }
         }
     } else {
@@ -621,11 +631,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulKernel(const __grid_constant
         clusterSync();
         if (finished) {
             if (g.outTag == T_F16) {
-                join<__half, BN>(g, stage0, rank, row, p0, q0, f);
+                join<__half, BN, NV>(g, stage0, rank, row, p0, q0, f);
             } else if (g.outTag == T_BF16) {
-                join<__nv_bfloat16, BN>(g, stage0, rank, row, p0, q0, f);
+                join<__nv_bfloat16, BN, NV>(g, stage0, rank, row, p0, q0, f);
             } else {
-                join<float, BN>(g, stage0, rank, row, p0, q0, f);
+                join<float, BN, NV>(g, stage0, rank, row, p0, q0, f);
             }
         }
         __syncwarp();
@@ -661,9 +671,9 @@ __device__ __forceinline__ void tileOf(const MxMatmulParams& g, int t, int* p, i
 // 32 columns of a warp's 32 rows -> the product, through shared memory and a bulk store: a row's 32 values are
 // 64 or 128 bytes, which leave together, where a thread's own stores of its row would be 16 bytes of 32
 // different rows at a time.
-template <class T>
+template <class T, bool NV>
 __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtensorMap* mapOut, unsigned int staging, int group, int lane,
-                                           long long row0, long long col0, const unsigned int r[32], const Factors& f) {
+                                           long long row0, long long col0, const unsigned int r[32], const Factors<NV>& f) {
     float v[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -719,9 +729,9 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
     }
 }
 
-template <class T>
+template <class T, bool NV>
 __device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, const CUtensorMap* mapOut, unsigned int staging, unsigned int acc, int buf,
-                                             long long row0, long long q0, const Factors& f, unsigned int accFree, int lane) {
+                                             long long row0, long long q0, const Factors<NV>& f, unsigned int accFree, int lane) {
     // columns 160..255 of tensor memory belong to both buffers: they are read first, and the next tile may start
     const int shared0 = buf ? 0 : 160;
     unsigned int r[3][32];
@@ -733,13 +743,13 @@ __device__ __forceinline__ void pairEpilogue(const MxMatmulParams& g, const CUte
     __syncwarp();
     if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(accFree) : "memory");
 #pragma unroll
-    for (int i = 0; i < 3; ++i) storeGroup<T>(g, mapOut, staging, i, lane, row0, q0 + shared0 + i * 32, r[i], f);
+    for (int i = 0; i < 3; ++i) storeGroup<T, NV>(g, mapOut, staging, i, lane, row0, q0 + shared0 + i * 32, r[i], f);
     const int rest = buf ? 96 : 0;
 #pragma unroll 1
     for (int i = 0; i < 5; ++i) {
         startRead(acc + rest + i * 32, r[0]);
         readsDone(r[0]);
-        storeGroup<T>(g, mapOut, staging, i + 3, lane, row0, q0 + rest + i * 32, r[0], f);
+        storeGroup<T, NV>(g, mapOut, staging, i + 3, lane, row0, q0 + rest + i * 32, r[0], f);
     }
 }
 
@@ -862,7 +872,7 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
             storeIn(smemAddr(&tilesDone), lane, whole);
         }
     } else if (warp < 4) {
-        const Factors f = factorsOf(g);
+        const Factors<NV> f = factorsOf<NV>(g);
         const unsigned int accFree0 = addrIn(accFree, 0);
         const unsigned int staging = stage0 + S::stages * S::stageBytes + warp * S::stagingBytes;
         int done = 0;
@@ -875,11 +885,11 @@ __global__ void __launch_bounds__(kThreads) mxMatmulPairKernel(const __grid_cons
             const unsigned int acc = tmem + buf * S::accStep + (static_cast<unsigned int>(warp * 32) << 16);
             const long long row0 = static_cast<long long>(tp) * 256 + rank * 128 + warp * 32, q0 = static_cast<long long>(tq) * 256;
             if (g.outTag == T_F16) {
-                pairEpilogue<__half>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
+                pairEpilogue<__half, NV>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
             } else if (g.outTag == T_BF16) {
-                pairEpilogue<__nv_bfloat16>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
+                pairEpilogue<__nv_bfloat16, NV>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
             } else {
-                pairEpilogue<float>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
+                pairEpilogue<float, NV>(g, &mapOut, staging, acc, buf, row0, q0, f, accFree0, lane);
             }
         }
     }
