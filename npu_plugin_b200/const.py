@@ -647,7 +647,8 @@ class CudaBackend:
     # ---- block-scaled 4-bit matrices (npu_plugin_b200.mx.MxMatrix; device pointers, on the backend's stream)
     def mx_quantize(self, src, dtype, src_ld, out, tensor_scale_given=False, values=None, values_ld=0):
         """src (rows x cols of `out`, f16/bf16/f32, src_ld elements between rows) -> the codes and scales of `out`;
-        `values` receives what they stand for, in the type of src."""
+        `values` receives what they stand for, in the type of src.  tensor_scale_given: nvfp4's is read, not found (mxfp4 has
+        none, whatever is said)."""
         rc = self.lib.b200c_mx_quantize(self.ctx, src, dtype, src_ld, out.ref, values, values_ld,
                                         A.MX_SCALE_GIVEN if tensor_scale_given and out.c.format == A.NVFP4 else 0)
         if rc:
@@ -942,7 +943,7 @@ class ContentAttr:
         """Block-scaled 4-bit floats (A.MXFP4 or A.NVFP4; no reference counterpart): the element type becomes F4E2M1, the
         blocks run along the innermost memory dimension, a multiple of 32.  The scales [rows, blocks] land in the
         returned attribute's `.mxScales`, for nvfp4 the tensor scale (found from the data when 0) and the largest
-        magnitude in `.mxTensorScale`."""
+        magnitude (0 when the scale is given) in `.mxTensorScale`."""
         mem = self._typeAt(A.X_QUANTIZE_MX).getMemShape()
         cols = mem[-1] if mem else 0
         rows = int(np.prod(mem[:-1], dtype=np.int64))

@@ -4,8 +4,9 @@
 // Four threads (mxfp4) or two (nvfp4) share a block and find its largest magnitude with shuffles.
 //
 // One pass over the data, bound by DRAM where the values are written, too: 11008 x 4096 f16 to mxfp4 with values
-// 29.9 us (6.85 TB/s of what the pass cannot do without), back to f16 18.5 us (6.2 TB/s).  Without the values it is instruction issue:
-// 23.6 us (4.9 TB/s), and 30.9 us for nvfp4, whose quotients take three instructions an element.
+// 33.6 us (6.1 TB/s of what the pass cannot do without), back to f16 19.0 us (6.0 TB/s).  Without the values it is instruction
+// issue: 23.2 us (4.9 TB/s, 18.0 million instructions in 71 % of the slots), and 32.6 us for nvfp4 (28.3 million in 74 %), whose
+// quotients take three instructions an element and whose blocks are half as long.
 #include "mx.h"
 #include "runtime.h"
 
@@ -476,7 +477,7 @@ __device__ __forceinline__ unsigned int topHere(const MxQuantParams& p, int thre
 // v / d in 32 bits, as codes and scales need it.  The method is Markstein's (Computation of elementary functions on the IBM
 // RISC System/6000 processor, IBM Journal of Research and Development 34, 1990): a reciprocal r by one Newton-Raphson
 // step, and the quotient q = v r corrected once by its remainder, q + (v - q d) r.  With the
-// division of the language instead 11008 x 4096 f16 to nvfp4, codes only, takes 45.5 us, not 32.5.
+// division of the language instead 11008 x 4096 f16 to nvfp4, codes only, takes 45.5 us, not 32.6.
 // With r off by 2^-23 at most (the approximation's error squared, and one rounding) q is off by 1.5 * 2^-23, and the sum
 // before its last rounding by the product of the two: less than 2^-44 of v / d.  That is less than correct rounding, but
 // enough for what is read from it, the side of a border between two codes or scales (or the border itself) that the rounded

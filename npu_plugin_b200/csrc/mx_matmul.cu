@@ -6,7 +6,7 @@
 // One side's rows are the 128 rows of a tile ("P"), the other's its columns ("Q").
 //
 // Two kernels.  mxMatmulPairKernel, for products of many tiles, is bound by the tensor pipe, and by power where it
-// runs long: 8192 x 4096 x 11008 (nvfp4) 124 us, 5.96 PFLOP/s -- 150 us in a long run, at 1000 W and 1.38 GHz.  Its tile of 256 x 256 for
+// runs long: 8192 x 4096 x 11008 (nvfp4) 125 us, 5.9 PFLOP/s -- 150 us in a long run, at 1000 W and 1.38 GHz.  Its tile of 256 x 256 for
 // two SMs is what the way from L2 allows: an SM takes 64 bytes a clock, and a 128 x 256 tile of one SM would need
 // 54 KB for 512 clocks of products, this one 38 KB.  mxMatmulKernel, for few rows on the left, is bound by that way from L2
 // and by latency: 1 x 11008 x 4096 (nvfp4) 6.4 us, 16 x 4096 x 11008 (mxfp4) 6.4 us, and with weights from DRAM
