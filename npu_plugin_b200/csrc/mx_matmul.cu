@@ -41,6 +41,7 @@ struct MxMatmulParams {
     long long ld;
     int outTag;            // T_F16, T_BF16, T_F32
     int wide;              // rows of the product are 16-byte aligned
+    int bulkTo;            // column that bulk stores may reach: of rows that end inside a 16-byte line they would fill the line with zeros
     int* err;
 };
 
@@ -668,6 +669,31 @@ __device__ __forceinline__ void tileOf(const MxMatmulParams& g, int t, int* p, i
     *p = group * G + (r - *q * high);
 }
 
+// 32 columns of a warp's 32 rows, staged as storeGroup() lays them, in rows that no bulk store can start at or end in: the
+// warp stores them one by one, 32 neighbours at a time.
+template <class T>
+__device__ __forceinline__ void storeRows(const MxMatmulParams& g, unsigned int at, int lane, long long row0, long long col0) {
+    constexpr int rowBytes = 32 * sizeof(T), chunks = rowBytes / 16;
+    const int rows = static_cast<int>(min(32ll, g.rowsP - row0));
+    T* out = static_cast<T*>(g.out) + row0 * g.ld + col0 + lane;
+    const bool mine = col0 + lane < g.rowsQ;
+    const int c = lane * static_cast<int>(sizeof(T)) / 16, in = lane * static_cast<int>(sizeof(T)) % 16;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i, out += g.ld) {
+        if (i < rows && mine) {
+            const unsigned int from = at + i * rowBytes + ((c ^ (chunks == 8 ? i & 7 : (i >> 1) & 3)) << 4) + in;
+            if (sizeof(T) == 2) {
+                unsigned short w;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+                *reinterpret_cast<unsigned short*>(out) = w;
+            } else {
+                unsigned int w;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+                *reinterpret_cast<unsigned int*>(out) = w;
+            }
+        }
+    }
+}
 // 32 columns of a warp's 32 rows -> the product, through shared memory and a bulk store: a row's 32 values are
 // 64 or 128 bytes, which leave together, where a thread's own stores of its row would be 16 bytes of 32
 // different rows at a time.
@@ -693,34 +719,20 @@ __device__ __forceinline__ void storeGroup(const MxMatmulParams& g, const CUtens
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
     }
     if (!g.wide) {
-        // rows that no bulk store can start at: the warp stores them one by one, 32 neighbours at a time
         __syncwarp();
-        const int rows = static_cast<int>(min(32ll, g.rowsP - row0));
-        T* out = static_cast<T*>(g.out) + row0 * g.ld + col0 + lane;
-        const bool mine = col0 + lane < g.rowsQ;
-        const int c = lane * static_cast<int>(sizeof(T)) / 16, in = lane * static_cast<int>(sizeof(T)) % 16;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i, out += g.ld) {
-            if (i < rows && mine) {
-                const unsigned int from = at + i * rowBytes + ((c ^ (chunks == 8 ? i & 7 : (i >> 1) & 3)) << 4) + in;
-                if (sizeof(T) == 2) {
-                    unsigned short w;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
-                    *reinterpret_cast<unsigned short*>(out) = w;
-                } else {
-                    unsigned int w;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
-                    *reinterpret_cast<unsigned int*>(out) = w;
-                }
-            }
-        }
+        storeRows<T>(g, at, lane, row0, col0);
         __syncwarp();
         return;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
+    const bool ends = col0 + 32 > g.bulkTo;  // inside a line
+    if (ends) {
+        storeRows<T>(g, at, lane, row0, col0);
+        __syncwarp();
+    }
     if (lane == 0) {
-        if (row0 < g.rowsP && col0 < g.rowsQ) {
+        if (row0 < g.rowsP && col0 < g.rowsQ && !ends) {
             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(mapOut),
                          "r"(static_cast<int>(col0)), "r"(static_cast<int>(row0)), "r"(at)
                          : "memory");
@@ -977,7 +989,8 @@ CUtensorMap scaleMapOf(const b200c_mx_matrix& m, int chunksPerTile, int boxTiles
     return map;
 }
 
-// The product as groups of 32 x 32 values; what lies behind its last row or column is not written.
+// The product as groups of 32 x 32 values; what lies behind its last row is not written, and behind its last column
+// nothing beyond that one's 16 bytes, which a bulk store fills up with zeros: MxMatmulParams::bulkTo keeps it from there.
 CUtensorMap outMapOf(void* out, int dtype, int64_t rows, int64_t cols, int64_t ld) {
     CUtensorMap map;
     const int es = dtBits(dtype) / 8;
@@ -1116,6 +1129,7 @@ void launchMxMatmul(Context* ctx, const b200c_mx_matrix& a, const b200c_mx_matri
     g.ld = outLd;
     g.outTag = dtype == B200C_F16 ? T_F16 : dtype == B200C_BF16 ? T_BF16 : T_F32;
     g.wide = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (outLd * es) % 16 == 0 && outLd * es < (int64_t(1) << 40);
+    g.bulkTo = q.rows * es % 16 != 0 ? static_cast<int>(q.rows) : 0x7FFFFFFF;
     g.err = ctx->errWord;
     if (pairs) {
         if (nv) {

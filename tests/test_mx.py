@@ -478,6 +478,25 @@ def test_matmul(dev, fmt, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(1507, 1789), (1600, 1785), (1601, 1792), (1537, 1704), (1600, 1808), (1537, 2057), (4900, 257), (129, 5001), (300, 1003),
+                                 (3, 129), (40, 700)])
+@pytest.mark.parametrize("k", [40, 700])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_matmul_writes_its_columns_alone(dev, fmt, m, n, k):
+    """Results inside a wider matrix whose rows are aligned: the columns behind the last, in its 16-byte line and
+    further, and the row behind the last stay as they were."""
+    (a, va), (b, vb) = random_held(fmt, m, k, m), random_held(fmt, n, k, n)
+    for dtype in TYPES:
+        line = 128 // torch.finfo(TYPES[dtype]).bits
+        for ld in (-(-n // line) * line, -(-n // line) * line + line):
+            out = torch.full((m * ld + 3 * line,), 7.0, dtype=TYPES[dtype], device="cuda")
+            dev.mx_matmul(a.m, b.m, out.data_ptr(), dtype, ld)
+            body, behind = out[:m * ld].view(m, ld), out[m * ld:]
+            check_product(body[:, :n].double().cpu().numpy(), va, vb, dtype)
+            assert (body[:, n:] == 7.0).all() and (behind == 7.0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(16, 256, 1024), (300, 700, 2048), (1600, 1800, 2048)])
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_matmul_is_exact_where_sums_are(dev, fmt, m, n, k):
